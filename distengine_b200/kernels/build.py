@@ -47,6 +47,8 @@ MODULES: dict[str, tuple[str, tuple[str, ...]]] = {
     "latent": ("latent.cu", ()),
     "experts": ("experts.cu", ()),
     "sublayer": ("sublayer.cu", ()),
+    "beam": ("beam.cu", ()),
+    "shared_prefix": ("shared_prefix.cu", ()),
 }
 
 

@@ -154,6 +154,16 @@ SIGNATURES: dict[str, dict[str, list]] = {
         "de_poly_norm": [I, P, I, P, P, I, I, I, F, P],
         "de_join_rmsnorm": [I, I, I, P, P, P, I, P, P, P, F, P, P, F, P, P, I, I, P],
     },
+    "beam": {
+        "de_beam_max_beams": [], "de_beam_max_take": [], "de_beam_scratch": [I, I, I, I],
+        "de_beam_select": [P, L, P, I, I, I, I, P, P, P, P, P],
+        "de_beam_reorder": [P, I, I, L, P, P, I, I, P, P],
+    },
+    "shared_prefix": {
+        "de_shared_rows_tile": [],
+        "de_shared_rows": [I, P, I, P, P, P, I, I, P, P, P, I, P, P, I, I, I, I, F, P, P],
+        "de_shared_merge": [I, P, I, P, P, P, P, I, I, I, I, P],
+    },
     "attention_decode": {
         "de_attn_decode_head_dim": [], "de_attn_decode_max_cluster": [],
         "de_attn_decode_blocks_per_sm": [I],

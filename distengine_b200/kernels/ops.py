@@ -74,6 +74,29 @@ def _i32(t: torch.Tensor, name: str) -> None:
           f"{name} must be a contiguous int32 CUDA tensor")
 
 
+def _on_device(*tensors: torch.Tensor) -> None:
+    """The tensors are on the current CUDA device, whose stream the launch goes to."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for t in tensors:
+        _need(t.is_cuda and t.device.index == here, "all tensors must be on the current CUDA device "
+              f"(cuda:{here}), got one on {t.device}")
+
+
+_status_words: dict[torch.device, torch.Tensor] = {}
+
+
+def _status_word(status: "torch.Tensor | None", like: torch.Tensor) -> torch.Tensor:
+    """The word in which a kernel records what it skipped: the caller's, or one of the device's."""
+    if status is not None:
+        _need(status.dtype == torch.int32 and status.numel() >= 1 and status.device == like.device,
+              "status must be an int32 tensor on the operands' device")
+        return status
+    word = _status_words.get(like.device)
+    if word is None:
+        word = _status_words[like.device] = torch.zeros(1, dtype=torch.int32, device=like.device)
+    return word
+
+
 # ------------------------------------------------------------------------------- embedding
 def embed_rows(ids: torch.Tensor, table: torch.Tensor, out: torch.Tensor,
                scale: float = 1.0) -> None:
@@ -729,3 +752,82 @@ def sample_rows(logits: torch.Tensor, out: torch.Tensor,
     lib = library.load("core")
     _check(lib.de_sample_rows(logits.data_ptr(), rows, vocab, _ptr(temperature), _ptr(seed),
                               _ptr(position), out.data_ptr(), _stream()), "sample_rows")
+
+
+# ------------------------------------------------------------------------------- beam search
+MAX_BEAMS, MAX_TAKE = 32, 64         # of ``csrc/beam.cu``
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, best: torch.Tensor, beam: torch.Tensor,
+                token: torch.Tensor, scratch: "torch.Tensor | None" = None) -> None:
+    """The next beams of every group: of the totals scores[g, b] + log_softmax(logits[g * beams + b])[v]
+    the ``take`` largest, best first, with their beams and tokens.
+
+    logits float32 [groups * beams, vocabulary] (row stride free), scores float32 [groups, beams];
+    best float32, beam and token int32, all [groups, take]; up to 32 beams, 64 taken.  Totals are formed
+    and compared in 64 bits; of equal ones the lower beam comes first, within a beam the larger logit,
+    then the lower token.  A total of minus infinity or NaN (a masked token, a dead beam, a row that
+    holds NaN or plus infinity) is no candidate; where too few are left, best is minus infinity and
+    beam and token are -1.  ``scratch``: uint8, ``beam_scratch`` bytes, used during the call."""
+    _need(logits.dim() == 2 and scores.dim() == 2 and best.dim() == 2,
+          "beam_select: logits [groups * beams, vocabulary], scores [groups, beams], best [groups, take]")
+    groups, beams = scores.shape
+    take, vocabulary = best.shape[1], logits.shape[1]
+    _need(logits.dtype == scores.dtype == best.dtype == torch.float32
+          and beam.dtype == token.dtype == torch.int32,
+          "beam_select: logits, scores and best are float32, beam and token int32")
+    _need(logits.shape[0] == groups * beams and best.shape == beam.shape == token.shape == (groups, take)
+          and scores.is_contiguous() and best.is_contiguous() and beam.is_contiguous()
+          and token.is_contiguous() and (vocabulary < 2 or logits.stride(1) == 1)
+          and (logits.shape[0] < 2 or logits.stride(0) >= vocabulary),
+          "beam_select: a row of logits a beam; contiguous scores, best, beam and token")
+    _need(1 <= beams <= MAX_BEAMS and 1 <= take <= MAX_TAKE and vocabulary >= 1,
+          f"beam_select: 1 to {MAX_BEAMS} beams, 1 to {MAX_TAKE} taken, a vocabulary")
+    _on_device(logits, scores, best, beam, token)
+    size = beam_scratch(groups, beams, vocabulary, take)
+    if groups == 0:
+        return
+    if scratch is None:
+        scratch = torch.empty(size, dtype=torch.uint8, device=logits.device)
+    _need(scratch.dtype == torch.uint8 and scratch.is_contiguous() and scratch.numel() >= size
+          and scratch.device == logits.device and scratch.data_ptr() % 16 == 0,
+          f"beam_select: scratch must be {size} bytes, 16-byte aligned")
+    lib = library.load("beam")
+    _check(lib.de_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), groups, beams,
+                              vocabulary, take, best.data_ptr(), beam.data_ptr(), token.data_ptr(),
+                              scratch.data_ptr(), _stream()), "beam_select")
+
+
+def beam_scratch(groups: int, beams: int, vocabulary: int, take: int) -> int:
+    """Bytes of scratch memory that ``beam_select`` uses for these sizes."""
+    size = int(library.load("beam").de_beam_scratch(groups, beams, vocabulary, take))
+    _need(size >= 0, f"beam_select: {groups} groups of {beams} beams over {vocabulary} tokens, "
+          f"{take} taken, are refused (code {size})")
+    return size
+
+
+def beam_reorder(rows: torch.Tensor, slots: torch.Tensor, parent: torch.Tensor,
+                 status: "torch.Tensor | None" = None) -> None:
+    """rows[:, slots[g, b]] <- rows[:, slots[g, parent[g, b]]] in place, for all beams at once: each
+    beam's row becomes what its parent's was before the call.
+
+    rows [layers, pool, ...] contiguous, of any dtype (recurrent states, pages of a cache); slots int32
+    [groups, beams]: each beam's row of the pool, all different (-1: a beam without one); parent int32
+    [groups, beams]: a beam of the same group (-1: the row stays as it is); up to 32 beams.  What cannot be used
+    stays as it is and sets ``status`` to 5: a slot or parent outside its range, the parent's missing
+    row, all of a group of which a row is named twice."""
+    _need(rows.dim() >= 2 and rows.is_contiguous(), "beam_reorder: rows [layers, pool, ...], contiguous")
+    _need(slots.dim() == 2 and slots.shape == parent.shape and slots.shape[1] <= MAX_BEAMS
+          and slots.dtype == parent.dtype == torch.int32 and slots.is_contiguous()
+          and parent.is_contiguous(), "beam_reorder: slots and parent int32 [groups, beams], "
+          f"contiguous, up to {MAX_BEAMS} beams")
+    _on_device(rows, slots, parent)
+    if rows.numel() == 0 or slots.numel() == 0:
+        return
+    status = _status_word(status, rows)
+    layers, pool = rows.shape[:2]
+    lib = library.load("beam")
+    _check(lib.de_beam_reorder(rows.data_ptr(), layers, pool,
+                               rows.numel() // (layers * pool) * rows.element_size(),
+                               slots.data_ptr(), parent.data_ptr(), slots.shape[0], slots.shape[1],
+                               status.data_ptr(), _stream()), "beam_reorder")
