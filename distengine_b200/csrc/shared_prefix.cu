@@ -23,11 +23,12 @@ namespace {
 
 using namespace shared_prefix;
 
-constexpr int ROWS = 8;               // query rows of a tile
+constexpr int ROWS = 8;               // query rows of a block
 constexpr int KT = 32;                // keys of a tile
 constexpr int THREADS = 128;
 
-// A warp owns two rows.  Scores: a lane a key; results: a lane every 32nd feature.
+// A block takes eight rows of an item (blockIdx.y: which), a warp two.  Scores: a lane a key;
+// results: a lane every 32nd feature.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 shared_rows_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ k_pages,
@@ -35,7 +36,8 @@ shared_rows_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ 
                    int table_stride, int num_pages, const int* __restrict__ seq_slot,
                    const int* __restrict__ seq_pos0, const Item* __restrict__ items,
                    float* __restrict__ partial_acc, float2* __restrict__ partial_ml, int heads,
-                   int kv_heads, int d, int page, float scale, int* __restrict__ status) {
+                   int kv_heads, int d, int page, float scale, int unit,
+                   int* __restrict__ status) {
     extern __shared__ float smem[];
     const int ld = d + 1;
     float* q_s = smem;                                    // [ROWS][d]
@@ -45,12 +47,14 @@ shared_rows_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ 
     const Item it = items[blockIdx.x / kv_heads];
     const int hk = blockIdx.x % kv_heads, g = heads / kv_heads;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int first = blockIdx.y * ROWS;                  // of the tile's rows
     pdl_wait();
-    const Range range = range_of(it, seq_pos0, ROWS, g, 1);
+    if (first >= it.count) return;
+    const Range range = range_of(it, seq_pos0, g, unit);
     const int slot = seq_slot[it.seq];
     for (int i = tid; i < ROWS * d; i += THREADS) {
-        const int r = it.row0 + i / d;
-        q_s[i] = r < it.rows ? to_float(q[(size_t)(it.tok0 + r / g) * q_stride +
+        const int r = it.row0 + first + i / d;
+        q_s[i] = first + i / d < it.count ? to_float(q[(size_t)(it.tok0 + r / g) * q_stride +
                                           (hk * g + r % g) * d + i % d])
                              : 0.0f;
     }
@@ -63,7 +67,7 @@ shared_rows_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ 
         for (int i = 0; i < 8; ++i) acc[r][i] = 0.0f;
     int hi[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) hi[r] = range.row_end(it, it.row0 + 2 * warp + r, g);
+    for (int r = 0; r < 2; ++r) hi[r] = range.row_end(it, first + 2 * warp + r, g);
 
     for (int kt = range.begin; kt < range.end; kt += KT) {
         __syncthreads();
@@ -116,8 +120,8 @@ shared_rows_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ 
     pdl_trigger();
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-        const int row = 2 * warp + r;
-        if (it.row0 + row >= it.rows) continue;
+        const int row = first + 2 * warp + r;
+        if (row >= it.count) continue;
         const size_t at = (size_t)(it.base + row) * kv_heads + hk;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -189,38 +193,38 @@ shared_merge_kernel(T* __restrict__ out, int out_stride, const int* __restrict__
 template <typename T>
 int rows_of(const void* q, int q_stride, const void* k_pages, const void* v_pages,
             const int* block_table, int table_stride, int num_pages, const int* seq_slot,
-            const int* seq_pos0, const int* items, int num_items, float* partial_acc,
-            float* partial_ml, int heads, int kv_heads, int d, int page, float scale, int* status,
-            cudaStream_t stream) {
+            const int* seq_pos0, const int* items, int num_items, int tile_rows, int unit,
+            float* partial_acc, float* partial_ml, int heads, int kv_heads, int d, int page,
+            float scale, int* status, cudaStream_t stream) {
     const int smem = (ROWS * d + 2 * KT * (d + 1)) * 4;
     if (smem > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(
             shared_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return (int)e;
     }
-    return de_launch(shared_rows_kernel<T>, dim3((unsigned)num_items * kv_heads), dim3(THREADS), smem,
-                     stream, (const T*)q, q_stride, (const T*)k_pages, (const T*)v_pages, block_table,
+    return de_launch(shared_rows_kernel<T>, dim3((unsigned)num_items * kv_heads, (tile_rows + ROWS - 1) / ROWS),
+                     dim3(THREADS), smem, stream, (const T*)q, q_stride, (const T*)k_pages, (const T*)v_pages, block_table,
                      table_stride, num_pages, seq_slot, seq_pos0, (const Item*)items, partial_acc,
-                     (float2*)partial_ml, heads, kv_heads, d, page, scale, status);
+                     (float2*)partial_ml, heads, kv_heads, d, page, scale, unit, status);
 }
 
 }  // namespace
 
-DE_EXPORT int de_shared_rows_tile() { return ROWS; }
-
+// `tile_rows`: most rows of an item; `unit`: what the ranges of own keys are a multiple of.
 DE_EXPORT int de_shared_rows(int dtype, const void* q, int q_stride, const void* k_pages,
                              const void* v_pages, const int* block_table, int table_stride,
                              int num_pages, const int* seq_slot, const int* seq_pos0,
-                             const int* items, int num_items, float* partial_acc, float* partial_ml,
-                             int heads, int kv_heads, int head_dim, int page, float scale,
-                             int* status, void* stream) {
+                             const int* items, int num_items, int tile_rows, int unit,
+                             float* partial_acc, float* partial_ml, int heads, int kv_heads,
+                             int head_dim, int page, float scale, int* status, void* stream) {
     if (num_items <= 0) return 0;
+    if (tile_rows < 1 || tile_rows > 1024 || unit < 1) return -3;
     if (head_dim < 2 || head_dim > 256 || head_dim % 2 || kv_heads < 1 || heads % kv_heads || page < 1 ||
         (long long)num_items * kv_heads > 0x7fffffffll)
         return -2;
     const auto f = dtype == DE_F32 ? rows_of<float> : rows_of<__nv_bfloat16>;
     return f(q, q_stride, k_pages, v_pages, block_table, table_stride, num_pages, seq_slot, seq_pos0,
-             items, num_items, partial_acc, partial_ml, heads, kv_heads, head_dim, page, scale, status,
+             items, num_items, tile_rows, unit, partial_acc, partial_ml, heads, kv_heads, head_dim, page, scale, status,
              (cudaStream_t)stream);
 }
 

@@ -11,7 +11,7 @@ namespace shared_prefix {
 // request for its own keys.
 struct Item {
     int tok0;        // the owner's first token
-    int rows;        // the owner's rows
+    int count;       // the tile's rows
     int row0;        // the tile's first row
     int seq;         // the request whose page table is read
     int begin;       // prefix: the range's first key; own keys: the prefix's length
@@ -31,17 +31,16 @@ struct Joined {
 struct Range {
     int begin, end;          // keys of the item
     int pos0;                // position of the owner's first token; prefix: beyond every key
-    // behind the last key that a row of the owner sees; rows that do not exist see none
-    __device__ __forceinline__ int row_end(const Item& it, int row, int g) const {
-        if (row >= it.rows) return begin;
-        return pos0 < 0 ? end : min(end, pos0 + row / g + 1);
+    // behind the last key that row i of the tile sees; rows that do not exist see none
+    __device__ __forceinline__ int row_end(const Item& it, int i, int g) const {
+        if (i >= it.count) return begin;
+        return pos0 < 0 ? end : min(end, pos0 + (it.row0 + i) / g + 1);
     }
 };
 
 // The keys of an item.  Own keys: from the prefix's end to the position of the tile's last token, in
 // `splits` ranges of a multiple of `unit` keys.
-__device__ __forceinline__ Range range_of(const Item& it, const int* seq_pos0, int tile_rows, int g,
-                                          int unit) {
+__device__ __forceinline__ Range range_of(const Item& it, const int* seq_pos0, int g, int unit) {
     Range r;
     if (it.end >= 0) {
         r.begin = it.begin;
@@ -50,8 +49,7 @@ __device__ __forceinline__ Range range_of(const Item& it, const int* seq_pos0, i
         return r;
     }
     r.pos0 = seq_pos0[it.seq];
-    const int last = min(it.row0 + tile_rows, it.rows) - 1;
-    const int stop = max(it.begin, r.pos0 + last / g + 1);
+    const int stop = max(it.begin, r.pos0 + (it.row0 + it.count - 1) / g + 1);
     const int splits = it.split >> 16, part = it.split & 0xffff;
     int each = (stop - it.begin + splits - 1) / splits;
     each = (each + unit - 1) / unit * unit;

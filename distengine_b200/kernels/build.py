@@ -49,6 +49,7 @@ MODULES: dict[str, tuple[str, tuple[str, ...]]] = {
     "sublayer": ("sublayer.cu", ()),
     "beam": ("beam.cu", ()),
     "shared_prefix": ("shared_prefix.cu", ()),
+    "shared_prefix_mma": ("shared_prefix_mma.cu", ()),  # built per head size: HEAD_DIM=<d>
 }
 
 

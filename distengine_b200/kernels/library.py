@@ -160,9 +160,12 @@ SIGNATURES: dict[str, dict[str, list]] = {
         "de_beam_reorder": [P, I, I, L, P, P, I, I, P, P],
     },
     "shared_prefix": {
-        "de_shared_rows_tile": [],
-        "de_shared_rows": [I, P, I, P, P, P, I, I, P, P, P, I, P, P, I, I, I, I, F, P, P],
+        "de_shared_rows": [I, P, I, P, P, P, I, I, P, P, P, I, I, I, P, P, I, I, I, I, F, P, P],
         "de_shared_merge": [I, P, I, P, P, P, P, I, I, I, I, P],
+    },
+    "shared_prefix_mma": {
+        "de_shared_mma_rows": [], "de_shared_mma_blocks_per_sm": [],
+        "de_shared_mma": [P, I, P, P, P, I, I, P, P, P, I, P, P, I, I, I, I, F, P, P],
     },
     "attention_decode": {
         "de_attn_decode_head_dim": [], "de_attn_decode_max_cluster": [],
@@ -184,13 +187,15 @@ def default_build_requests() -> list[tuple[str, tuple[str, ...]]]:
     """Every module; the per-head-size attention for the head sizes of common models."""
     requests = [(module, ()) for module in _build.MODULES
                 if module in SIGNATURES
-                and module not in ("attention_mma", "attention_decode", "attention_tcgen05")]
+                and module not in ("attention_mma", "attention_decode", "attention_tcgen05",
+                                   "shared_prefix_mma")]
     # (16 and 32: what the tiny models that the smoke test generates with have)
     return (requests + [("attention_mma", (f"HEAD_DIM={d}",)) for d in (16, 64, 128)]
             + [("attention_mma", ("HEAD_DIM=32", "SPLIT_WEIGHTS=1"))]
             + [("attention_mma", (f"HEAD_DIM={d}", "SPLIT_WEIGHTS=1", "SCORE_EXTRAS=1"))
                for d in (16, 32, 64, 128)]
             + [("attention_tcgen05", (f"HEAD_DIM={d}",)) for d in (64, 128)]
+            + [("shared_prefix_mma", (f"HEAD_DIM={d}",)) for d in (16, 64, 128)]
             + [("attention_decode", (f"HEAD_DIM={d}",)) for d in (16, 64, 128)])
 
 

@@ -19,7 +19,7 @@ import numpy as np
 import torch
 
 from . import library
-from .attention import check_head_dim
+from .attention import check_head_dim, uses_tensor_cores
 from .ops import _check, _need, _on_device, _status_word, _stream, _tag
 
 MAX_SPLITS = 256
@@ -28,9 +28,10 @@ MAX_SPLITS = 256
 @dataclass
 class SharedPlan:
     """The work lists of a step's requests: ``items`` by kernel, int32 [n, 8] (``shared_prefix::
-    Item``), ``seqs`` int32 [requests, 8] (``shared_prefix::Joined``), ``token_seq`` int32 [tokens];
+    Item``; ``shapes``: their most rows and the unit of their ranges), ``seqs`` int32 [requests, 8] (``shared_prefix::Joined``), ``token_seq`` int32 [tokens];
     ``partial_rows`` rows of partial results.  The arrays are numpy's until ``to`` moves them."""
     items: dict
+    shapes: dict
     seqs: "np.ndarray | torch.Tensor"
     token_seq: "np.ndarray | torch.Tensor"
     partial_rows: int
@@ -40,14 +41,14 @@ class SharedPlan:
     def to(self, device: "torch.device | str") -> "SharedPlan":
         move = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(device)
         seqs = move(self.seqs)
-        return SharedPlan({name: move(a) for name, a in self.items.items()}, seqs,
+        return SharedPlan({name: move(a) for name, a in self.items.items()}, self.shapes, seqs,
                           move(self.token_seq), self.partial_rows, self.tokens, seqs.device)
 
 
 @dataclass(frozen=True)
 class Tile:
-    """A kernel's tile: its name among the plan's items, query rows, keys that a range is a multiple of,
-    blocks that fill the device."""
+    """A tile of a kernel: the kernel's name among the plan's items, query rows, keys that a range is a
+    multiple of (one number for all tiles of a kernel), blocks that fill the device."""
     name: str
     rows: int
     unit: int
@@ -81,7 +82,12 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
     seqs = np.zeros((len(qlen), 8), dtype=np.int64)
     seqs[:, 0], seqs[:, 1] = tok0, np.repeat(group_tok0, sizes)
     items: dict[str, list] = {}
+    shapes: dict[str, tuple] = {}
     base = 0
+
+    def add(t: Tile, part: np.ndarray) -> None:
+        items.setdefault(t.name, []).append(part)
+        shapes[t.name] = (max(t.rows, shapes.get(t.name, (0, 0))[0]), t.unit)
 
     # shared keys: ranges of one length for all groups, so long that the blocks fill the device once
     tiles = [prefix_tile(int(t) * group) for t in group_tokens]
@@ -99,12 +105,13 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
         count = -(-rows // t.rows)
         tile, chunk = np.divmod(np.arange(count * chunks), chunks)
         part = np.zeros((count * chunks, 8), dtype=np.int64)
-        part[:, 0], part[:, 1], part[:, 2] = group_tok0[g], rows, tile * t.rows
+        part[:, 0], part[:, 2] = group_tok0[g], tile * t.rows
+        part[:, 1] = np.minimum(t.rows, rows - part[:, 2])
         part[:, 3], part[:, 4] = first[g], chunk * each
         part[:, 5] = np.minimum(p, (chunk + 1) * each)
         part[:, 7] = base + (tile * chunks + chunk) * t.rows
         # a range after the other, its tiles side by side: they read the same keys
-        items.setdefault(t.name, []).append(part[np.argsort(chunk, kind="stable")])
+        add(t, part[np.argsort(chunk, kind="stable")])
         members_of = slice(int(first[g]), int(first[g] + sizes[g]))
         seqs[members_of, 2], seqs[members_of, 3], seqs[members_of, 4] = base, chunks, t.rows
         base += count * chunks * t.rows
@@ -131,15 +138,16 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
             tile, split = at // splits[owner], at % splits[owner]
             start = base + np.cumsum(n * t.rows) - n * t.rows
             part = np.zeros((len(owner), 8), dtype=np.int64)
-            part[:, 0], part[:, 1], part[:, 2] = tok0[s[owner]], rows[owner], tile * t.rows
+            part[:, 0], part[:, 2] = tok0[s[owner]], tile * t.rows
+            part[:, 1] = np.minimum(t.rows, rows[owner] - part[:, 2])
             part[:, 3], part[:, 4], part[:, 5] = s[owner], np.repeat(prefix, sizes)[s[owner]], -1
             part[:, 6] = split | splits[owner] << 16
             part[:, 7] = start[owner] + (tile * splits[owner] + split) * t.rows
-            items.setdefault(t.name, []).append(part)
+            add(t, part)
             seqs[s, 5], seqs[s, 6], seqs[s, 7] = start, splits, t.rows
             base += int((n * t.rows).sum())
     _need(base < 1 << 31, "shared prefix: too many partial results")
-    return SharedPlan({name: np.concatenate(parts) for name, parts in items.items()}, seqs,
+    return SharedPlan({name: np.concatenate(parts) for name, parts in items.items()}, shapes, seqs,
                       np.repeat(np.arange(len(qlen)), qlen), base, total)
 
 
@@ -158,6 +166,8 @@ class SharedPrefixAttention:
             raise ValueError(f"shared prefix: the scale must be positive, got {scale}")
         self.dtype, self.heads, self.kv_heads, self.head_dim = dtype, heads, kv_heads, head_dim
         self.scale, self.group = float(scale), heads // kv_heads
+        self.tensor_cores = uses_tensor_cores(dtype, head_dim)
+        self.mma_module = ("shared_prefix_mma", (f"HEAD_DIM={head_dim}",))
         self._device = None if device is None else torch.device(device)
         self._sms: "int | None" = None
 
@@ -170,7 +180,13 @@ class SharedPrefixAttention:
 
     def tiles(self) -> "tuple":
         """(rows of a group -> ``Tile``, rows of a request -> ``Tile``)."""
-        plain = Tile("rows", 8, 32, 4 * self._sm_count())
+        sms = self._sm_count()
+        if self.tensor_cores:
+            lib = library.load(*self.mma_module)
+            most, blocks = lib.de_shared_mma_rows(), lib.de_shared_mma_blocks_per_sm() * sms
+            tile = lambda rows: Tile("mma", min(most, max(1, -(-rows // 16)) * 16), 64, blocks)
+            return tile, tile
+        plain = Tile("rows", 8, 32, 4 * sms)
         return (lambda rows: plain), (lambda rows: plain)
 
     def host_plan(self, seq_qlen, group_sizes, prefix_lens, tail: int = 0) -> SharedPlan:
@@ -224,13 +240,22 @@ class SharedPrefixAttention:
         ml = make("shared_prefix.partial_ml", (rows * 2,), torch.float32)
         lib = library.load("shared_prefix")
         tag = _tag(q.dtype)
+        # (rows that are not in 4-byte pieces, pages that are not in 16-byte ones: one by one)
+        aligned = not (q.stride(0) % 2 or q.data_ptr() % 4 or k_pages.data_ptr() % 16
+                       or v_pages.data_ptr() % 16)
         for name, items in plan.items.items():
-            _check(lib.de_shared_rows(
-                tag, q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
-                block_table.data_ptr(), block_table.stride(0), k_pages.shape[0],
-                seq_slot.data_ptr(), seq_pos0.data_ptr(), items.data_ptr(), items.shape[0],
-                acc.data_ptr(), ml.data_ptr(), self.heads, self.kv_heads, d, k_pages.shape[2],
-                self.scale, status.data_ptr(), _stream()), "shared prefix attention")
+            rows, unit = plan.shapes[name]
+            before = (q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
+                      block_table.data_ptr(), block_table.stride(0), k_pages.shape[0],
+                      seq_slot.data_ptr(), seq_pos0.data_ptr(), items.data_ptr(), items.shape[0])
+            behind = (acc.data_ptr(), ml.data_ptr(), self.heads, self.kv_heads, d, k_pages.shape[2],
+                      self.scale, status.data_ptr(), _stream())
+            if name == "mma" and aligned:
+                _check(library.load(*self.mma_module).de_shared_mma(*before, *behind),
+                       "shared prefix attention (mma)")
+            else:
+                _check(lib.de_shared_rows(tag, *before, rows, unit, *behind),
+                       "shared prefix attention")
         _check(lib.de_shared_merge(tag, out.data_ptr(), out.stride(0), plan.token_seq.data_ptr(),
                                    plan.seqs.data_ptr(), acc.data_ptr(), ml.data_ptr(), tokens,
                                    self.heads, self.kv_heads, d, _stream()), "shared prefix merge")

@@ -37,10 +37,10 @@ def _seen(plan, tiles, group, kv_heads, qlen, sizes, prefix, own):
     for name, items in plan.items.items():
         t = rows_of[name]
         for it in items.tolist():
-            at, rows, row0, seq, begin, end, split, base = it
-            assert row0 < rows and 0 <= base and base + t.rows <= plan.partial_rows
+            at, n, row0, seq, begin, end, split, base = it
+            assert 0 < n <= t.rows and 0 <= base and base + t.rows <= plan.partial_rows
+            assert plan.shapes[name] == (t.rows, t.unit)
             used[base: base + t.rows] += 1
-            n = min(t.rows, rows - row0)
             if end < 0:                               # as range_of in the kernels' header
                 assert at == tok0[seq]
                 stop = max(begin, pos0[seq] + (row0 + n - 1) // group + 1)
