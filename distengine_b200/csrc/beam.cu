@@ -43,30 +43,34 @@ constexpr int MAX_VOCAB = 1 << 27;
 typedef unsigned long long u64;
 
 constexpr int SLICE_THREADS = 512;
+constexpr int FOUND = 512;             // keys that a block keeps of its slice, to pick the best from
+constexpr int QUADS = 4;               // 16-byte loads of a thread under way at once
+constexpr int SEGMENTS = 2048;
+constexpr int WINNERS = 320;           // segments that are looked at again
 constexpr int JOIN_THREADS = 512;
+constexpr int PICKS = 256;             // candidates of which the best are picked
 constexpr double UNSURE = 2.2e-6;      // totals of two beams nearer than this are formed again
 constexpr float COARSE = 1048576.0f;   // rows with a larger maximum: formed in 64 bits at once
 constexpr float LOG2E = 1.4426950408889634f;
 
+__device__ __forceinline__ unsigned ordered(float v) {    // of a number that is not NaN
+    const unsigned u = __float_as_uint(v);
+    return u ^ (unsigned)((int)u >> 31 | 0x80000000);
+}
 __device__ __forceinline__ u64 logit_key(float v, int token) {
     if (!(v > -INFINITY)) return 0;                       // NaN and minus infinity
-    const unsigned u = __float_as_uint(v + 0.0f);         // (minus zero is as large as zero)
-    const unsigned ordered = u & 0x80000000u ? ~u : u | 0x80000000u;
-    return (u64)ordered << 32 | (unsigned)~token;
+    return (u64)ordered(v + 0.0f) << 32 | (unsigned)~token;        // (minus zero is as large as zero)
 }
 __device__ __forceinline__ float key_logit(u64 key) {
-    const unsigned ordered = (unsigned)(key >> 32);
-    return __uint_as_float(ordered & 0x80000000u ? ordered & 0x7fffffffu : ~ordered);
+    const unsigned u = (unsigned)(key >> 32);
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 __device__ __forceinline__ int key_token(u64 key) { return (int)~(unsigned)key; }
 
-__device__ __forceinline__ u64 shfl_max(u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
-        v = w > v ? w : v;
-    }
-    return v;
+__device__ __forceinline__ u64 warp_largest(u64 v) {      // upper halves first, then the lower ones of those
+    const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32));
+    const unsigned low = (unsigned)(v >> 32) == high ? (unsigned)v : 0;
+    return (u64)high << 32 | __reduce_max_sync(0xffffffffu, low);
 }
 __device__ __forceinline__ double shfl_sum(double v) {
 #pragma unroll
@@ -89,14 +93,23 @@ __device__ __forceinline__ float exponent_of(float top) {
 }
 
 // A threshold with which `count(t)`, the number of keys of at least t over the block, lies between
-// `want` and `most`; 1 if there are at most `most` keys that are not 0 in all.  Halves the range
-// of the keys until it is met, which distinct keys guarantee for most >= want.  `count` is called
-// by all threads; `top` is the largest key.
+// `want` and `most`, or all keys but 0 where there are at most `most`.  `low` is a guess from below
+// (1: none), `top` the largest key; the range between is halved until it is met, which distinct keys
+// guarantee for most >= want (keys that are the same end with the largest threshold that has
+// `want`).  `count` is called by all threads.
 template <typename Count>
-__device__ __forceinline__ u64 threshold(u64 top, int want, int most, Count count) {
-    if (top == 0 || count(1) <= most) return 1;
-    u64 low = 1, high = top;                              // count(low) > most, and high not below it
-    while (low < high) {
+__device__ __forceinline__ u64 threshold(u64 low, u64 top, int want, int most, Count count) {
+    u64 high = top;
+    if (low > 1) {
+        const int n = count(low);
+        if (n >= want && n <= most) return low;
+        if (n < want) { high = low - 1; low = 1; }
+    }
+    if (low <= 1) {
+        if (top == 0 || count(1) <= most) return 1;
+        low = 1;
+    }
+    while (low < high) {                                  // count(low) > most
         const u64 mid = low + ((high - low + 1) >> 1);
         const int n = count(mid);
         if (n >= want) {
@@ -109,117 +122,259 @@ __device__ __forceinline__ u64 threshold(u64 top, int want, int most, Count coun
     return low;
 }
 
-// A slice goes by in pieces of four logits (one 16-byte load); up to three logits before the first
-// 16-byte boundary and behind the last are pieces of their own.
-struct Pieces {
-    const float* x;          // the slice
-    int n, head, quads;      // logits; those before the boundary; whole pieces
-    __device__ __forceinline__ Pieces(const float* p, int count) : x(p), n(count) {
-        head = min(n, (int)((16 - ((uintptr_t)p & 15)) & 15) >> 2);
-        quads = (n - head) >> 2;
+// For each of n things, how many come before it: eight threads count for one.  `before(c, j)`, then
+// `place(c, rank)` by one thread.
+template <int THREADS, typename Before, typename Place>
+__device__ __forceinline__ void rank_all(int n, Before before, Place place) {
+    const int sub = threadIdx.x & 7;
+    for (int first = 0; first < n; first += THREADS / 8) {
+        const int c = first + (threadIdx.x >> 3);
+        int rank = 0;
+        if (c < n)
+            for (int j = sub; j < n; j += 8) rank += before(c, j) ? 1 : 0;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        if (sub == 0 && c < n) place(c, rank);
     }
-    __device__ __forceinline__ int count() const { return quads + 2; }
-    // piece i: 0 .. quads - 1 whole ones, quads the head, quads + 1 the rest; -inf where there is none
-    __device__ __forceinline__ float4 get(int i) const {
-        if (i < quads) return __ldg(reinterpret_cast<const float4*>(x + head) + i);
+}
+
+// A slice goes by in quads (four logits, a 16-byte load); up to three logits before the first 16-byte
+// boundary and up to three behind the last quad are for themselves.  For the search of the best, runs
+// of 2^shift quads form segments; segment 0 is the head, the last one the rest.
+struct Quads {
+    const float* x;          // the slice
+    int n, head, count;      // logits; those before the boundary; whole quads
+    int shift;               // the smallest segments of which there are not too many
+    __device__ __forceinline__ Quads(const float* p, int logits) : x(p), n(logits) {
+        head = min(n, (int)((16 - ((uintptr_t)p & 15)) & 15) >> 2);
+        count = (n - head) >> 2;
+        shift = 0;
+        while ((count - 1) >> shift > SEGMENTS - 3) shift += shift == 0 ? 3 : shift == 3 ? 2 : 1;
+    }
+    __device__ __forceinline__ float4 quad(int i) const {
+        return *(reinterpret_cast<const float4*>(x + head) + i);
+    }
+    __device__ __forceinline__ int segments() const { return ((count - 1) >> shift) + 3; }
+    // logits of the head (0) or the rest (1), minus infinity where there is none
+    __device__ __forceinline__ float4 edge(int which) const {
+        const int first = edge_start(which), most = which ? n - first : head;
         float v[4];
-        const int first = start(i), most = i == quads ? head : i == quads + 1 ? n - first : 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = j < most ? x[first + j] : -INFINITY;
         return make_float4(v[0], v[1], v[2], v[3]);
     }
-    __device__ __forceinline__ int start(int i) const {
-        return i < quads ? head + 4 * i : i == quads ? 0 : head + 4 * quads;
-    }
+    __device__ __forceinline__ int edge_start(int which) const { return which ? head + 4 * count : 0; }
+};
+// (never NaN: the largest number, or minus infinity)
+__device__ __forceinline__ float largest(const float4& v) {
+    return fmaxf(fmaxf(fmaxf(v.x, v.y), v.z), fmaxf(v.w, -INFINITY));
+}
+constexpr unsigned NOTHING = 0x007fffffu;                 // ordered(-INFINITY)
+
+template <int N> struct Int {
+    static constexpr int value = N;
 };
 
-__global__ void __launch_bounds__(SLICE_THREADS)
+// One pass over the slice: the sum, and the maximum of every segment.  A segment whose maximum is not
+// among the `take` largest holds none of the `take` best, so only as many segments are looked at
+// again (1.5% of a row of 128,256, still in the L2 for the most part).
+__global__ void __launch_bounds__(SLICE_THREADS, 4)
 beam_slices_kernel(const float* __restrict__ logits, long long stride, int vocab, int slice,
                    int slices, int take, float* __restrict__ maxima, double* __restrict__ sums,
                    u64* __restrict__ keys) {
-    extern __shared__ u64 found[];                        // [2 take x logits of a thread]
-    __shared__ u64 warp_top[SLICE_THREADS / 32];
+    __shared__ u64 found[FOUND];
+    __shared__ unsigned segment_s[SEGMENTS];
+    __shared__ unsigned part_top[SLICE_THREADS / 8];
     __shared__ double warp_sum_s[SLICE_THREADS / 32];
-    __shared__ int count_s;
+    __shared__ int winner_s[WINNERS], winners_s, count_s, counts_s[3];
     const int row = blockIdx.x / slices, part = blockIdx.x % slices;
     const int begin = part * slice;
-    const Pieces pieces(logits + (long long)row * stride + begin, min(vocab, begin + slice) - begin);
-    const int count = pieces.count();
+    const Quads quads(logits + (long long)row * stride + begin, min(vocab, begin + slice) - begin);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int shift = quads.shift, segments = quads.segments();
     if (tid == 0) count_s = 0;
+    if (tid < 3) counts_s[tid] = 0;
+    if (shift > 5) {                                      // several warps' loads form a segment
+        for (int i = tid; i < segments; i += SLICE_THREADS) segment_s[i] = 0;
+        __syncthreads();
+    }
     pdl_wait();
-    // the largest logit and the first piece that holds it; the sum of 2^(logit log2(e) - r)
+    // the sum of 2^(logit log2(e) - r), with an r near the largest so far
     float top_v = -INFINITY, r = 0.0f;
-    int top_piece = -1;
     double sum = 0.0;
-    for (int i = tid; i < count; i += 4 * SLICE_THREADS) {
-        float4 v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            v[u] = i + u * SLICE_THREADS < count
-                       ? pieces.get(i + u * SLICE_THREADS)
-                       : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        const float before = top_v;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float m = fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w));
-            if (m > top_v) { top_v = m; top_piece = i + u * SLICE_THREADS; }
-        }
-        if (top_v > before && (before == -INFINITY || top_v * LOG2E > r + 1.0f)) {
-            const float to = exponent_of(top_v);
+    auto follow = [&](float m) {
+        if (!(m > top_v)) return;
+        if (top_v == -INFINITY || m * LOG2E > r + 1.0f) {
+            const float to = exponent_of(m);
             sum *= power_of_two(r - to);                  // (0 when there was nothing before)
             r = to;
         }
-        float part_sum[4];
+        top_v = m;
+    };
+    auto terms = [&](const float4& v) {
+        return (exp2_fast(fmaf(v.x, LOG2E, -r)) + exp2_fast(fmaf(v.y, LOG2E, -r))) +
+               (exp2_fast(fmaf(v.z, LOG2E, -r)) + exp2_fast(fmaf(v.w, LOG2E, -r)));
+    };
+    // LANES of a warp form a segment; 33: more than a warp
+    auto go_through = [&](auto lanes) {
+        constexpr int LANES = decltype(lanes)::value;
+        const float4* p = reinterpret_cast<const float4*>(quads.x + quads.head) + tid;
+        auto step = [&](int base, const float4 (&v)[QUADS], int left) {
+            float m[QUADS];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            part_sum[u] = (exp2_fast(fmaf(v[u].x, LOG2E, -r)) + exp2_fast(fmaf(v[u].y, LOG2E, -r))) +
-                          (exp2_fast(fmaf(v[u].z, LOG2E, -r)) + exp2_fast(fmaf(v[u].w, LOG2E, -r)));
-        sum += (double)((part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]));
-    }
-    u64 mine = 0;
-    if (top_piece >= 0) {
-        const float4 v = pieces.get(top_piece);
-        const float e[4] = {v.x, v.y, v.z, v.w};
-        int at = 3;
+            for (int u = 0; u < QUADS; ++u) m[u] = largest(v[u]);
+            follow(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
 #pragma unroll
-        for (int j = 3; j >= 0; --j)
-            if (e[j] == top_v) at = j;
-        mine = logit_key(top_v, begin + pieces.start(top_piece) + at);
+            for (int u = 0; u < QUADS; ++u) {
+                unsigned o = ordered(m[u] + 0.0f);
+                if (LANES == 8) {
+#pragma unroll
+                    for (int d = 1; d < 8; d <<= 1) o = max(o, __shfl_xor_sync(0xffffffffu, o, d));
+                } else if (LANES >= 32) {
+                    o = __reduce_max_sync(0xffffffffu, o);
+                }
+                const int i = base + u * SLICE_THREADS + tid;
+                if (u * SLICE_THREADS < left && (LANES == 1 || lane % (LANES < 32 ? LANES : 32) == 0)) {
+                    if (LANES > 32) atomicMax(&segment_s[1 + (i >> shift)], o);
+                    else segment_s[1 + i / LANES] = o;
+                }
+            }
+            sum += (double)((terms(v[0]) + terms(v[1])) + (terms(v[2]) + terms(v[3])));
+        };
+        int base = 0;
+        for (; base + QUADS * SLICE_THREADS <= quads.count; base += QUADS * SLICE_THREADS) {
+            float4 v[QUADS];
+#pragma unroll
+            for (int u = 0; u < QUADS; ++u) v[u] = p[base + u * SLICE_THREADS];
+            step(base, v, QUADS * SLICE_THREADS);
+        }
+        if (base < quads.count) {
+            float4 v[QUADS];
+#pragma unroll
+            for (int u = 0; u < QUADS; ++u)
+                v[u] = base + u * SLICE_THREADS + tid < quads.count
+                           ? p[base + u * SLICE_THREADS]
+                           : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            step(base, v, quads.count - base - tid);
+        }
+    };
+    if (shift == 0) go_through(Int<1>());
+    else if (shift == 3) go_through(Int<8>());
+    else if (shift == 5) go_through(Int<32>());
+    else go_through(Int<33>());
+    if (tid < 2) {
+        const float4 v = quads.edge(tid);
+        const float m = largest(v);
+        follow(m);
+        segment_s[tid ? segments - 1 : 0] = ordered(m + 0.0f);
+        sum += (double)terms(v);
     }
-    u64 top = shfl_max(mine);
-    if (lane == 0) warp_top[warp] = top;
     __syncthreads();
-    top = 0;
-    for (int w = 0; w < SLICE_THREADS / 32; ++w) top = max(top, warp_top[w]);
-    const float m = top ? key_logit(top) : -INFINITY;
+    // The largest; and a guess at the last of the `take` largest segments: as many parts of the block as
+    // are taken have each a segment of at least the smallest part's largest.
+    unsigned mine = 0;
+    for (int i = tid; i < segments; i += SLICE_THREADS) mine = max(mine, segment_s[i]);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+    if ((lane & 7) == 0) part_top[tid >> 3] = mine;
+    __syncthreads();
+    const unsigned x = part_top[2 * lane], y = part_top[2 * lane + 1];
+    unsigned guess = take > 32 ? min(x, y) : max(x, y);
+    if (take <= 16) guess = max(guess, __shfl_xor_sync(0xffffffffu, guess, 1));
+    guess = __reduce_min_sync(0xffffffffu, guess);
+    const unsigned top = __reduce_max_sync(0xffffffffu, max(x, y));
+    const float m = top > NOTHING ? key_logit((u64)top << 32) : -INFINITY;
+
     sum = shfl_sum(sum * power_of_two(r - exponent_of(m)));
     if (lane == 0) warp_sum_s[warp] = sum;
 
-    // the threads whose largest key is below the threshold have none of the best; the others look again
-    const u64 floor_key = threshold(top, min(take, SLICE_THREADS), 2 * take, [&](u64 t) {
-        return __syncthreads_count(mine >= t);
-    });
-    if (mine >= floor_key)
-        for (int i = tid; i < count; i += SLICE_THREADS) {
-            const float4 v = pieces.get(i);
+    // Segments with at least the guess's maximum are few enough nearly always.  Where they are not,
+    // segments are told apart by their maxima and, equal ones, by their place.
+    auto segment_key = [&](int i) {
+        const unsigned o = segment_s[i];
+        return o > NOTHING ? (u64)o << 32 | (unsigned)~i : 0;
+    };
+    int turn = 0;                                         // one barrier a count: three counters in turn
+    auto segments_from = [&](u64 t) {
+        int k = 0;
+        for (int i = tid; i < segments; i += SLICE_THREADS) k += segment_key(i) >= t;
+        k = __reduce_add_sync(0xffffffffu, k);
+        if (lane == 0 && k) atomicAdd(&counts_s[turn], k);
+        __syncthreads();
+        k = counts_s[turn];
+        turn = turn == 2 ? 0 : turn + 1;
+        if (tid == 0) counts_s[turn == 2 ? 0 : turn + 1] = 0;
+        return k;
+    };
+    const u64 last = threshold(guess > NOTHING ? (u64)guess << 32 : 1, (u64)top << 32 | 0xffffffffu, take,
+                               min(max(6 * take, 96), WINNERS), segments_from);
+    if (tid == 0) winners_s = 0;
+    __syncthreads();
+    for (int i = tid; i < segments; i += SLICE_THREADS)
+        if (segment_key(i) >= last) winner_s[atomicAdd(&winners_s, 1)] = i;
+    __syncthreads();
+    // The keys of at least t in those segments, all their quads side by side; how many there are.
+    auto collect = [&](u64 t) {
+        float floor_v = key_logit(t);
+        if (floor_v != floor_v) floor_v = -INFINITY;      // (a threshold below all numbers)
+        auto keep = [&](const float4& v, int first) {
             const float e[4] = {v.x, v.y, v.z, v.w};
-            const int first = begin + pieces.start(i);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const u64 k = logit_key(e[j], first + j);
-                if (k >= floor_key) found[atomicAdd(&count_s, 1)] = k;
+                const u64 k = logit_key(e[j], begin + first + j);
+                if (k < t || k == 0) continue;
+                const int at = atomicAdd(&count_s, 1);
+                if (at < FOUND) found[at] = k;
+            }
+        };
+        const int all = winners_s << shift;
+        for (int base = tid; base < all; base += QUADS * SLICE_THREADS) {
+            float4 v[QUADS];
+            int first[QUADS];
+#pragma unroll
+            for (int u = 0; u < QUADS; ++u) {
+                const int at = base + u * SLICE_THREADS;
+                first[u] = -1;
+                if (at >= all) continue;
+                const int s = winner_s[at >> shift], q = at & ((1 << shift) - 1);
+                const int i = ((s - 1) << shift) + q;
+                if (s == 0 || s == segments - 1) {
+                    if (q) continue;
+                    v[u] = quads.edge(s != 0);
+                    first[u] = quads.edge_start(s != 0);
+                } else if (i < quads.count) {
+                    v[u] = quads.quad(i);
+                    first[u] = quads.head + 4 * i;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < QUADS; ++u)
+                if (first[u] >= 0 && largest(v[u]) >= floor_v) keep(v[u], first[u]);
+        }
+        __syncthreads();
+        return count_s;
+    };
+    u64 low = last >> 32 << 32, high = (u64)top << 32 | 0xffffffffu;
+    int n = collect(low);
+    if (n > FOUND)                                        // the best are crowded in few segments
+        while (low < high) {
+            const u64 mid = low + ((high - low + 1) >> 1);
+            __syncthreads();
+            if (tid == 0) count_s = 0;
+            __syncthreads();
+            n = collect(mid);
+            if (n >= take) {
+                low = mid;
+                if (n <= FOUND) break;
+            } else {
+                high = mid - 1;
             }
         }
-    __syncthreads();
     pdl_trigger();
-    const int n = count_s;
     u64* out = keys + (size_t)blockIdx.x * take;
-    for (int c = tid; c < n; c += SLICE_THREADS) {
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += found[j] > found[c];
+    rank_all<SLICE_THREADS>(n, [&](int c, int j) { return found[j] > found[c]; }, [&](int c, int rank) {
         if (rank < take) out[rank] = found[c];
-    }
+    });
     for (int c = n + tid; c < take; c += SLICE_THREADS) out[c] = 0;
     if (tid == 0) {
         double all = 0.0;
@@ -245,30 +400,45 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
                  const float* __restrict__ maxima, const double* __restrict__ sums,
                  const u64* __restrict__ keys, float* __restrict__ best, int* __restrict__ beam,
                  int* __restrict__ token) {
-    extern __shared__ u64 total_s[];                      // [beams x slices x take]
+    extern __shared__ u64 total_s[];                      // [beams x slices x take], twice
+    u64* key_s = total_s + beams * slices * take;
     __shared__ double max_s[MAX_BEAMS], log_s[MAX_BEAMS]; // log(sum exp) of a row: max + log
-    __shared__ u64 warp_part[JOIN_THREADS / 32];
-    __shared__ int warp_count[JOIN_THREADS / 32];
-    __shared__ int pick_s[2 * MAX_TAKE + 2], order_s[MAX_TAKE + 1];
+    __shared__ u64 warp_part[2][JOIN_THREADS / 32];
+    __shared__ int counts_s[3];
+    __shared__ int pick_s[PICKS], order_s[MAX_TAKE + 1];
+    __shared__ u64 pick_total_s[PICKS];
+    __shared__ float score_s[MAX_BEAMS];
     __shared__ int count_s;
     __shared__ unsigned again_s;                          // rows whose sums are to be formed again
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) again_s = 0;
+    if (tid < 3) counts_s[tid] = 0;
     __syncthreads();
+    const int per_beam = slices * take, n = beams * per_beam;
+    const u64* mine = keys + (size_t)g * n;
     pdl_wait();
     pdl_trigger();
+    if (tid < beams) score_s[tid] = scores[(size_t)g * beams + tid];
+    for (int c = tid; c < n; c += JOIN_THREADS)           // (while the rows' sums are on their way)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(
+                         (unsigned)__cvta_generic_to_shared(key_s + c)), "l"(mine + c) : "memory");
     for (int b = warp; b < beams; b += JOIN_THREADS / 32) {
         const size_t at = ((size_t)g * beams + b) * slices;
+        // (a lane's sum refers to the exponent of its own slices' maximum, as the threads' did)
         float m = -INFINITY;
-        for (int s = lane; s < slices; s += 32) m = fmaxf(m, maxima[at + s]);
+        double sum = 0.0;
+        auto shrink = [](float e) { return e < -1000.0f ? 0.0 : power_of_two(e); };
+        for (int s = lane; s < slices; s += 32) {
+            const float x = maxima[at + s];
+            const double y = sums[at + s], top = fmaxf(m, x);
+            sum = (sum != 0.0 ? sum * shrink(exponent_of(m) - exponent_of(top)) : 0.0) +
+                  (y != 0.0 ? y * shrink(exponent_of(x) - exponent_of(top)) : 0.0);
+            m = top;
+        }
+        const float own = exponent_of(m);
         m = warp_max(m);
         const float r = exponent_of(m);
-        double sum = 0.0;
-        for (int s = lane; s < slices; s += 32) {
-            const float e = exponent_of(maxima[at + s]) - r;
-            if (sums[at + s] != 0.0) sum += sums[at + s] * (e < -1000.0f ? 0.0 : power_of_two(e));
-        }
-        sum = shfl_sum(sum);
+        sum = shfl_sum(sum != 0.0 ? sum * shrink(own - r) : 0.0);
         if (lane == 0) {
             // (a float32 log2(e) makes the logits larger by a factor, which is taken back for the
             // largest: what is left is the factor on the others' distance from it)
@@ -279,32 +449,32 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
                 atomicOr(&again_s, 1u << b);
         }
     }
-    const int per_beam = slices * take, n = beams * per_beam;
-    const u64* mine = keys + (size_t)g * n;
     // (the logit less the row's maximum first: both may be the lowest number there is)
     auto total_of = [&](int c) {
         const int b = c / per_beam;
-        return (double)scores[(size_t)g * beams + b] +
-               (((double)key_logit(mine[c]) - max_s[b]) - log_s[b]);
+        return (double)score_s[b] +
+               (((double)key_logit(key_s[c]) - max_s[b]) - log_s[b]);
     };
+    int turn = 0;                             // one barrier a count: three counters in turn
     auto over_block = [&](auto test) {
         int k = 0;
         for (int c = tid; c < n; c += JOIN_THREADS) k += test(c) ? 1 : 0;
         k = __reduce_add_sync(0xffffffffu, k);
+        if (lane == 0) atomicAdd(&counts_s[turn], k);
         __syncthreads();
-        if (lane == 0) warp_count[warp] = k;
-        __syncthreads();
-        k = 0;
-        for (int w = 0; w < JOIN_THREADS / 32; ++w) k += warp_count[w];
+        k = counts_s[turn];
+        turn = turn == 2 ? 0 : turn + 1;
+        if (tid == 0) counts_s[turn == 2 ? 0 : turn + 1] = 0;
         return k;
     };
     auto place = [&](int c) {                 // of equal totals: beam, larger logit, lower token
-        const u64 k = mine[c];
+        const u64 k = key_s[c];
         return (u64)(c / per_beam) << 59 | (u64)(unsigned)~(unsigned)(k >> 32) << 27 |
                (unsigned)key_token(k);
     };
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
     // one more than is taken: what the last one taken is compared with
-    const int want = take + 1, most = 2 * want;
+    const int want = take + 1, most = max(2 * want, 96);
     unsigned formed = 0;                                  // rows whose sums are 64-bit ones
     int found;
     for (;;) {
@@ -323,30 +493,38 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
                 sum += (u64)__double2ll_rn(exp((double)x[i] - m) * unit);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane == 0) warp_part[warp] = sum;
+            if (lane == 0) warp_part[0][warp] = sum;
             __syncthreads();
             if (tid == 0) {
                 sum = 0;
-                for (int w = 0; w < JOIN_THREADS / 32; ++w) sum += warp_part[w];
+                for (int w = 0; w < JOIN_THREADS / 32; ++w) sum += warp_part[0][w];
                 log_s[b] = log((double)sum / unit);
             }
             __syncthreads();
         }
-        u64 top = 0;
+        // the largest, and a guess at the last one wanted: the largest last one of a slice
+        u64 top = 0, guess = 0;
         for (int c = tid; c < n; c += JOIN_THREADS) {
-            const u64 t = mine[c] ? total_key(total_of(c)) : 0;
+            const u64 t = key_s[c] ? total_key(total_of(c)) : 0;
             total_s[c] = t;
-            top = t > top ? t : top;
+            top = max(top, t);
         }
-        top = shfl_max(top);
-        if (lane == 0) warp_part[warp] = top;
+        for (int i = tid; i < beams * slices; i += JOIN_THREADS) {
+            const int c = i * take + take - 1;
+            if (key_s[c]) guess = max(guess, total_key(total_of(c)));
+        }
+        top = warp_largest(top);
+        guess = warp_largest(guess);
+        if (lane == 0) { warp_part[0][warp] = top; warp_part[1][warp] = guess; }
         if (tid == 0) count_s = 0;
         __syncthreads();
-        top = 0;
-        for (int w = 0; w < JOIN_THREADS / 32; ++w) top = max(top, warp_part[w]);
+        for (int w = 0; w < JOIN_THREADS / 32; ++w) {
+            top = max(top, warp_part[0][w]);
+            guess = max(guess, warp_part[1][w]);
+        }
 
         // the best by their totals; of those with the total of the last place the first by `place`
-        const u64 t0 = threshold(top, want, most, [&](u64 t) {
+        const u64 t0 = threshold(guess, top, want, most, [&](u64 t) {
             return over_block([&](int c) { return total_s[c] >= t; });
         });
         u64 last = ~0ull;
@@ -362,19 +540,20 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
         }
         for (int c = tid; c < n; c += JOIN_THREADS) {
             const u64 t = total_s[c];
-            if (t > t0 || (t == t0 && t != 0 && place(c) <= last)) pick_s[atomicAdd(&count_s, 1)] = c;
+            if (t > t0 || (t == t0 && t != 0 && place(c) <= last)) {
+                const int at = atomicAdd(&count_s, 1);
+                pick_s[at] = c;
+                pick_total_s[at] = t;
+            }
         }
         __syncthreads();
         found = count_s;
-        for (int i = tid; i < found; i += JOIN_THREADS) {
-            const int c = pick_s[i];
-            int rank = 0;
-            for (int j = 0; j < found; ++j) {
-                const int d = pick_s[j];
-                rank += total_s[d] > total_s[c] || (total_s[d] == total_s[c] && place(d) < place(c));
-            }
-            if (rank < want) order_s[rank] = c;
-        }
+        rank_all<JOIN_THREADS>(found, [&](int i, int j) {
+            const u64 x = pick_total_s[i], y = pick_total_s[j];
+            return y > x || (y == x && place(pick_s[j]) < place(pick_s[i]));
+        }, [&](int i, int rank) {
+            if (rank < want) order_s[rank] = pick_s[i];
+        });
         __syncthreads();
         found = min(found, want);
         // neighbours of different beams that are too near each other for the sums that they have
@@ -393,25 +572,26 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
         const int c = i < found ? order_s[i] : -1;
         best[at] = c < 0 ? -INFINITY : (float)key_total(total_s[c]);
         beam[at] = c < 0 ? -1 : c / per_beam;
-        token[at] = c < 0 ? -1 : key_token(mine[c]);
+        token[at] = c < 0 ? -1 : key_token(key_s[c]);
     }
 }
 
-// slices a row is cut into, and elements of one
+// Slices that a row is cut into, and their logits: as many blocks as the SMs hold at once (four each),
+// of no fewer than 2,048 logits.  (512 rows of 128,256 in one slice each, 512 blocks; in four, whose
+// ends of a few microseconds are then paid four times, 73 us instead of SELECT_LARGE.)
 struct Slicing {
-    int slices, elements, per_thread;
+    int slices, elements;
 };
 constexpr int JOIN_MOST = 8192;                           // candidates of a group in shared memory
 Slicing slicing(int rows, int beams, int vocab, int take) {
-    const int blocks = 4 * 148;
-    int slices = (vocab + 64 * SLICE_THREADS - 1) / (64 * SLICE_THREADS);
-    while (rows * slices < blocks && vocab / (slices + 1) >= 4 * SLICE_THREADS) ++slices;
-    const int most = JOIN_MOST / (beams * take);
-    if (slices > most) slices = most < 1 ? 1 : most;
+    int slices = rows > 0 ? 4 * 148 / rows : 1;
+    const int least = vocab / (4 * SLICE_THREADS), most = JOIN_MOST / (beams * take);
+    if (slices > least) slices = least;
+    if (slices > most) slices = most;
+    if (slices < 1) slices = 1;
     Slicing s;
     s.elements = (vocab + slices - 1) / slices;
     s.slices = (vocab + s.elements - 1) / s.elements;
-    s.per_thread = 4 * ((s.elements / 4 + 2 + SLICE_THREADS - 1) / SLICE_THREADS);
     return s;
 }
 size_t aligned(size_t bytes) { return (bytes + 15) & ~(size_t)15; }
@@ -421,18 +601,25 @@ size_t aligned(size_t bytes) { return (bytes + 15) & ~(size_t)15; }
 // group in one layer: it reads the pieces of every row that a moved beam takes, and only then writes,
 // so the rows can change places without a buffer.
 // ------------------------------------------------------------------------------------------
+#ifndef REORDER_BLOCKS
+#define REORDER_BLOCKS 16
+#endif
 constexpr int MOVE_THREADS = 256;
+
+// pieces of a row that a thread has under way at once: as many as 64 registers hold for all beams
+template <typename U, int BEAMS> __host__ __device__ constexpr int pieces_at_once() {
+    const int n = 256 / (BEAMS * (int)sizeof(U));
+    return n < 1 ? 1 : n > 8 ? 8 : n;
+}
 
 template <typename U, int BEAMS>
 __global__ void __launch_bounds__(MOVE_THREADS)
 beam_reorder_kernel(unsigned char* __restrict__ x, long long row_bytes, int pool,
                     const int* __restrict__ slots, const int* __restrict__ parent, int groups,
-                    int beams, int blocks_per_row, int* __restrict__ status) {
+                    int beams, int chunks, int units, int* __restrict__ status) {
+    constexpr int N = pieces_at_once<U, BEAMS>();
     __shared__ int from_s[BEAMS], to_s[BEAMS], slot_s[BEAMS];
-    const int block = blockIdx.x % blocks_per_row;
-    const int g = blockIdx.x / blocks_per_row % groups;
-    const long long layer = blockIdx.x / blocks_per_row / groups;
-    const int tid = threadIdx.x;
+    const int g = blockIdx.y, tid = threadIdx.x;
     pdl_wait();
     pdl_trigger();
     if (tid < BEAMS) slot_s[tid] = tid < beams ? slots[g * beams + tid] : -1;
@@ -462,26 +649,44 @@ beam_reorder_kernel(unsigned char* __restrict__ x, long long row_bytes, int pool
         to_s[tid] = to;
     }
     __syncthreads();
-    const long long at = ((long long)block * MOVE_THREADS + tid) * sizeof(U);
-    if (at >= row_bytes) return;
-    unsigned char* base = x + layer * pool * row_bytes + at;
-    U v[BEAMS];
+    // a chunk is N pieces of every thread; layer after layer, the blocks of the group in turn
+    for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const long long at = ((long long)(unit % chunks) * N * MOVE_THREADS + tid) * sizeof(U);
+        unsigned char* base = x + (long long)(unit / chunks) * pool * row_bytes + at;
+        U v[BEAMS][N];
 #pragma unroll
-    for (int b = 0; b < BEAMS; ++b)
-        if (from_s[b] >= 0) v[b] = *reinterpret_cast<const U*>(base + from_s[b] * row_bytes);
+        for (int b = 0; b < BEAMS; ++b) {
+            if (from_s[b] < 0) continue;
+            const unsigned char* src = base + from_s[b] * row_bytes;
 #pragma unroll
-    for (int b = 0; b < BEAMS; ++b)
-        if (from_s[b] >= 0) *reinterpret_cast<U*>(base + to_s[b] * row_bytes) = v[b];
+            for (int n = 0; n < N; ++n)
+                if (at + n * MOVE_THREADS * (long long)sizeof(U) < row_bytes)
+                    v[b][n] = *reinterpret_cast<const U*>(src + n * MOVE_THREADS * sizeof(U));
+        }
+#pragma unroll
+        for (int b = 0; b < BEAMS; ++b) {
+            if (from_s[b] < 0) continue;
+            unsigned char* dst = base + to_s[b] * row_bytes;
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                if (at + n * MOVE_THREADS * (long long)sizeof(U) < row_bytes)
+                    *reinterpret_cast<U*>(dst + n * MOVE_THREADS * sizeof(U)) = v[b][n];
+        }
+    }
 }
 
 template <typename U, int BEAMS>
 int reorder_with(unsigned char* x, int layers, int pool, long long row_bytes, const int* slots,
                  const int* parent, int groups, int beams, int* status, cudaStream_t stream) {
-    const long long per_row = (row_bytes / (long long)sizeof(U) + MOVE_THREADS - 1) / MOVE_THREADS;
-    const long long blocks = per_row * groups * layers;
-    if (blocks > 0x7fffffffll) return -4;
-    return de_launch(beam_reorder_kernel<U, BEAMS>, dim3((unsigned)blocks), dim3(MOVE_THREADS), 0,
-                     stream, x, row_bytes, pool, slots, parent, groups, beams, (int)per_row, status);
+    const long long per_chunk = pieces_at_once<U, BEAMS>() * MOVE_THREADS * (long long)sizeof(U);
+    const long long chunks = (row_bytes + per_chunk - 1) / per_chunk, units = chunks * layers;
+    if (units > 0x7fffffffll || groups > 65535) return -4;
+    // a block looks the group's moves up once and goes through several chunks
+    long long blocks = (REORDER_BLOCKS * 148 + groups - 1) / groups;
+    if (blocks > units) blocks = units;
+    return de_launch(beam_reorder_kernel<U, BEAMS>, dim3((unsigned)blocks, groups), dim3(MOVE_THREADS),
+                     0, stream, x, row_bytes, pool, slots, parent, groups, beams, (int)chunks,
+                     (int)units, status);
 }
 template <typename U>
 int reorder_of(unsigned char* x, int layers, int pool, long long row_bytes, const int* slots,
@@ -506,7 +711,6 @@ DE_EXPORT int de_beam_scratch(int groups, int beams, int vocab, int take) {
         vocab > MAX_VOCAB || (long long)groups * beams > (1 << 20))
         return -2;
     const Slicing s = slicing(groups * beams, beams, vocab, take);
-    if ((size_t)2 * take * s.per_thread * 8 > 200 * 1024) return -3;
     const size_t n = (size_t)groups * beams * s.slices;
     const size_t bytes = aligned(4 * n) + aligned(8 * n) + 8 * n * take;
     return bytes > 0x7fffffff ? -4 : (int)bytes;
@@ -523,14 +727,13 @@ DE_EXPORT int de_beam_select(const float* logits, long long stride, const float*
     float* maxima = (float*)scratch;
     double* sums = (double*)((char*)scratch + aligned(4 * n));
     u64* keys = (u64*)((char*)sums + aligned(8 * n));
-    const int found = 2 * take * s.per_thread * 8, totals = beams * s.slices * take * 8;
-    cudaError_t e = cudaSuccess;
-    if (found > 32 * 1024)
-        e = cudaFuncSetAttribute(beam_slices_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, found);
-    if (e == cudaSuccess && totals > 32 * 1024)
-        e = cudaFuncSetAttribute(beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, totals);
-    if (e != cudaSuccess) return (int)e;
-    const int code = de_launch(beam_slices_kernel, dim3((unsigned)n), dim3(SLICE_THREADS), found,
+    const int totals = 2 * beams * s.slices * take * 8;
+    if (totals > 32 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(
+            beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, totals);
+        if (e != cudaSuccess) return (int)e;
+    }
+    const int code = de_launch(beam_slices_kernel, dim3((unsigned)n), dim3(SLICE_THREADS), 0,
                                (cudaStream_t)stream, logits, stride, vocab, s.elements, s.slices, take,
                                maxima, sums, keys);
     if (code) return code;

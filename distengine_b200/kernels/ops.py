@@ -6,6 +6,7 @@ model code.
 
 from __future__ import annotations
 
+import functools
 import os
 
 import torch
@@ -76,10 +77,14 @@ def _i32(t: torch.Tensor, name: str) -> None:
 
 def _on_device(*tensors: torch.Tensor) -> None:
     """The tensors are on the current CUDA device, whose stream the launch goes to."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else None
+    here = tensors[0].get_device()
     for t in tensors:
-        _need(t.is_cuda and t.device.index == here, "all tensors must be on the current CUDA device "
-              f"(cuda:{here}), got one on {t.device}")
+        if t.get_device() != here or here < 0:
+            raise ValueError("all tensors must be on the current CUDA device, got one on "
+                             f"{t.device} beside one on {tensors[0].device}")
+    if here != torch.cuda.current_device():
+        raise ValueError(f"all tensors must be on the current CUDA device, got one on cuda:{here} "
+                         f"while cuda:{torch.cuda.current_device()} is current")
 
 
 _status_words: dict[torch.device, torch.Tensor] = {}
@@ -781,28 +786,31 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, best: torch.Tensor, 
           and token.is_contiguous() and (vocabulary < 2 or logits.stride(1) == 1)
           and (logits.shape[0] < 2 or logits.stride(0) >= vocabulary),
           "beam_select: a row of logits a beam; contiguous scores, best, beam and token")
-    _need(1 <= beams <= MAX_BEAMS and 1 <= take <= MAX_TAKE and vocabulary >= 1,
-          f"beam_select: 1 to {MAX_BEAMS} beams, 1 to {MAX_TAKE} taken, a vocabulary")
+    if not (1 <= beams <= MAX_BEAMS and 1 <= take <= MAX_TAKE and vocabulary >= 1):
+        raise ValueError(f"beam_select: 1 to {MAX_BEAMS} beams, 1 to {MAX_TAKE} taken, a vocabulary; "
+                         f"got {beams}, {take} and {vocabulary}")
     _on_device(logits, scores, best, beam, token)
     size = beam_scratch(groups, beams, vocabulary, take)
     if groups == 0:
         return
     if scratch is None:
         scratch = torch.empty(size, dtype=torch.uint8, device=logits.device)
-    _need(scratch.dtype == torch.uint8 and scratch.is_contiguous() and scratch.numel() >= size
-          and scratch.device == logits.device and scratch.data_ptr() % 16 == 0,
-          f"beam_select: scratch must be {size} bytes, 16-byte aligned")
+    elif (scratch.dtype != torch.uint8 or not scratch.is_contiguous() or scratch.numel() < size
+          or scratch.device != logits.device or scratch.data_ptr() % 16):
+        raise ValueError(f"beam_select: scratch must be {size} bytes (uint8), 16-byte aligned")
     lib = library.load("beam")
     _check(lib.de_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), groups, beams,
                               vocabulary, take, best.data_ptr(), beam.data_ptr(), token.data_ptr(),
                               scratch.data_ptr(), _stream()), "beam_select")
 
 
+@functools.lru_cache(maxsize=1024)
 def beam_scratch(groups: int, beams: int, vocabulary: int, take: int) -> int:
     """Bytes of scratch memory that ``beam_select`` uses for these sizes."""
     size = int(library.load("beam").de_beam_scratch(groups, beams, vocabulary, take))
-    _need(size >= 0, f"beam_select: {groups} groups of {beams} beams over {vocabulary} tokens, "
-          f"{take} taken, are refused (code {size})")
+    if size < 0:
+        raise ValueError(f"beam_select: {groups} groups of {beams} beams over {vocabulary} tokens, "
+                         f"{take} taken, are refused (code {size})")
     return size
 
 
