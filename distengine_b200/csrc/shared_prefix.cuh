@@ -4,7 +4,14 @@
 
 #include "common.cuh"
 
+// The kernels of a step do not depend on one another, and each lets its successor start once its own
+// wait for its predecessor has returned.  So those behind the first (`behind`) need not wait before they
+// begin: what the step reads was complete when the first one's wait returned.  They wait before they
+// end instead, so that what waits for them has waited for all.
+
 namespace shared_prefix {
+
+constexpr int HALF_ROWS = 128;
 
 // A tile of query rows with a range of keys.  Rows are (token, query head of the kv head's group),
 // counted from the first token of the owner: all requests of a group for keys of its prefix, one
@@ -16,7 +23,8 @@ struct Item {
     int seq;         // the request whose page table is read
     int begin;       // prefix: the range's first key; own keys: the prefix's length
     int end;         // prefix: behind the range's last key; own keys: -1
-    int split;       // own keys: which of `splits` equal ranges this is, | splits << 16
+    int split;       // own keys: which of `splits` equal ranges this is, | splits << 16;
+                     // prefix: 1 where the range has two places for up to HALF_ROWS rows each
     int base;        // the tile's place among the partial results, in rows
 };
 
@@ -57,6 +65,9 @@ __device__ __forceinline__ Range range_of(const Item& it, const int* seq_pos0, i
     r.end = min(stop, r.begin + each);
     return r;
 }
+
+// The second place of a range that has two, by a kernel that needs one: no key.
+__device__ __forceinline__ bool has_second_place(const Item& it) { return it.end >= 0 && it.split; }
 
 // A page of a request; -1, with the status set, where it has none.
 __device__ __forceinline__ int page_of(const int* block_table, int table_stride, int num_pages,

@@ -47,17 +47,26 @@ shared_mma_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
                   int table_stride, int num_pages, const int* __restrict__ seq_slot,
                   const int* __restrict__ seq_pos0, const Item* __restrict__ items,
                   float* __restrict__ partial_acc, float2* __restrict__ partial_ml, int heads,
-                  int kv_heads, int page, float scale, int* __restrict__ status) {
+                  int kv_heads, int page, float scale, int behind, int* __restrict__ status) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int gid = lane >> 2, tig = lane & 3;
-    const Item it = items[blockIdx.x / kv_heads];
+    Item it = items[blockIdx.x / kv_heads];
     const int hk = blockIdx.x % kv_heads, g = heads / kv_heads;
+    const bool second = has_second_place(it);
+    if (!behind) pdl_wait();
+    const Range range = range_of(it, seq_pos0, g, UNIT);
+    // of an item with more rows than a block takes, the block's
+    it.row0 += blockIdx.y * ROWS;
+    it.base += blockIdx.y * ROWS;
+    it.count = min(ROWS, it.count - (int)blockIdx.y * ROWS);
+    if (it.count <= 0) {
+        if (behind) pdl_wait();
+        return;
+    }
     const int live = (it.count + 15) >> 4;                // row tiles that hold rows
     __nv_bfloat16* ring = reinterpret_cast<__nv_bfloat16*>(smem_raw) + warp * STAGES * STAGE;
 
-    pdl_wait();
-    const Range range = range_of(it, seq_pos0, g, UNIT);
     const int slot = seq_slot[it.seq];
     const int tiles = (range.end - range.begin + NK - 1) / NK;
     const int mine = tiles > warp ? (tiles - warp + WARPS - 1) / WARPS : 0;
@@ -321,9 +330,14 @@ shared_mma_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             }
             const size_t at = (size_t)(it.base + rt * 16 + r) * kv_heads + hk;
             *reinterpret_cast<float4*>(partial_acc + at * D + f) = a;
-            if (f == 0) partial_ml[at] = make_float2(top, l);
+            if (f == 0) {
+                partial_ml[at] = make_float2(top, l);
+                if (second)
+                    partial_ml[at + (size_t)HALF_ROWS * kv_heads] = make_float2(-INFINITY, 0.0f);
+            }
         }
     }
+    if (behind) pdl_wait();
 }
 
 }  // namespace
@@ -334,13 +348,15 @@ DE_EXPORT int de_shared_mma_blocks_per_sm() {
     return 227 * 1024 / (SMEM + 1024) < 4 ? 227 * 1024 / (SMEM + 1024) : 4;
 }
 
-// Items of up to de_shared_mma_rows() rows; q in 4-byte pieces, pages in 16-byte ones.
+// `tile_rows`: most rows of an item (above de_shared_mma_rows() in several blocks); `behind` as in
+// shared_prefix.cu; q in 4-byte pieces, pages in 16-byte ones.
 DE_EXPORT int de_shared_mma(const void* q, int q_stride, const void* k_pages, const void* v_pages,
                             const int* block_table, int table_stride, int num_pages,
                             const int* seq_slot, const int* seq_pos0, const int* items, int num_items,
-                            float* partial_acc, float* partial_ml, int heads, int kv_heads,
+                            int tile_rows, int behind, float* partial_acc, float* partial_ml, int heads, int kv_heads,
                             int head_dim, int page, float scale, int* status, void* stream) {
     if (num_items <= 0) return 0;
+    if (tile_rows < 1 || tile_rows > 1024) return -3;
     if (head_dim != D || kv_heads < 1 || heads % kv_heads || page < 1 ||
         (long long)num_items * kv_heads > 0x7fffffffll)
         return -2;
@@ -351,9 +367,10 @@ DE_EXPORT int de_shared_mma(const void* q, int q_stride, const void* k_pages, co
             shared_mma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return (int)e;
     }
-    return de_launch(shared_mma_kernel, dim3((unsigned)num_items * kv_heads), dim3(THREADS), SMEM,
+    return de_launch(shared_mma_kernel, dim3((unsigned)num_items * kv_heads, (tile_rows + ROWS - 1) / ROWS),
+                     dim3(THREADS), SMEM,
                      (cudaStream_t)stream, (const __nv_bfloat16*)q, q_stride,
                      (const __nv_bfloat16*)k_pages, (const __nv_bfloat16*)v_pages, block_table,
                      table_stride, num_pages, seq_slot, seq_pos0, (const Item*)items, partial_acc,
-                     (float2*)partial_ml, heads, kv_heads, page, scale, status);
+                     (float2*)partial_ml, heads, kv_heads, page, scale, behind, status);
 }

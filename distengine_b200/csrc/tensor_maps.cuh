@@ -44,6 +44,22 @@ struct Key {
 // A [rows, cols] bfloat16 matrix with row stride ld (elements), boxes of box_rows x box_cols,
 // 128-byte swizzle, zero fill outside.  0 or a negative code (-20: no driver entry point, -21:
 // the driver refused the map).
+inline int make(CUtensorMap* map, const void* base, long long rows, int cols, int ld, int box_rows,
+                int box_cols) {
+    EncodeTiled encode = encode_fn();
+    if (encode == nullptr) return -20;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+    cuuint32_t elem[2] = {1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base),
+                              dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : -21;
+}
+
+// `make`, but a map that was made before comes from the table.
 inline int get(CUtensorMap* map, const void* base, long long rows, int cols, int ld, int box_rows,
                int box_cols) {
     constexpr int SLOTS = 256;
@@ -58,17 +74,8 @@ inline int get(CUtensorMap* map, const void* base, long long rows, int cols, int
             *map = maps[i];
             return 0;
         }
-    EncodeTiled encode = encode_fn();
-    if (encode == nullptr) return -20;
-    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
-    cuuint32_t elem[2] = {1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base),
-                              dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return -21;
+    const int code = make(map, base, rows, cols, ld, box_rows, box_cols);
+    if (code) return code;
     const int slot = used < SLOTS ? used++ : (next++ % SLOTS);
     keys[slot] = key;
     maps[slot] = *map;

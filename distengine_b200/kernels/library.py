@@ -160,12 +160,16 @@ SIGNATURES: dict[str, dict[str, list]] = {
         "de_beam_reorder": [P, I, I, L, P, P, I, I, P, P],
     },
     "shared_prefix": {
-        "de_shared_rows": [I, P, I, P, P, P, I, I, P, P, P, I, I, I, P, P, I, I, I, I, F, P, P],
+        "de_shared_rows": [I, P, I, P, P, P, I, I, P, P, P, I, I, I, I, P, P, I, I, I, I, F, P, P],
         "de_shared_merge": [I, P, I, P, P, P, P, I, I, I, I, P],
     },
     "shared_prefix_mma": {
         "de_shared_mma_rows": [], "de_shared_mma_blocks_per_sm": [],
-        "de_shared_mma": [P, I, P, P, P, I, I, P, P, P, I, P, P, I, I, I, I, F, P, P],
+        "de_shared_mma": [P, I, P, P, P, I, I, P, P, P, I, I, I, P, P, I, I, I, I, F, P, P],
+    },
+    "shared_prefix_tcgen05": {
+        "de_shared_tcgen05_page_ok": [I],
+        "de_shared_tcgen05": [P, I, P, P, P, I, I, P, P, P, I, P, P, I, I, I, I, F, P, P],
     },
     "attention_decode": {
         "de_attn_decode_head_dim": [], "de_attn_decode_max_cluster": [],
@@ -188,7 +192,7 @@ def default_build_requests() -> list[tuple[str, tuple[str, ...]]]:
     requests = [(module, ()) for module in _build.MODULES
                 if module in SIGNATURES
                 and module not in ("attention_mma", "attention_decode", "attention_tcgen05",
-                                   "shared_prefix_mma")]
+                                   "shared_prefix_mma", "shared_prefix_tcgen05")]
     # (16 and 32: what the tiny models that the smoke test generates with have)
     return (requests + [("attention_mma", (f"HEAD_DIM={d}",)) for d in (16, 64, 128)]
             + [("attention_mma", ("HEAD_DIM=32", "SPLIT_WEIGHTS=1"))]
@@ -196,6 +200,7 @@ def default_build_requests() -> list[tuple[str, tuple[str, ...]]]:
                for d in (16, 32, 64, 128)]
             + [("attention_tcgen05", (f"HEAD_DIM={d}",)) for d in (64, 128)]
             + [("shared_prefix_mma", (f"HEAD_DIM={d}",)) for d in (16, 64, 128)]
+            + [("shared_prefix_tcgen05", (f"HEAD_DIM={d}",)) for d in (64, 128)]
             + [("attention_decode", (f"HEAD_DIM={d}",)) for d in (16, 64, 128)])
 
 

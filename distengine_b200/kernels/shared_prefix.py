@@ -48,11 +48,39 @@ class SharedPlan:
 @dataclass(frozen=True)
 class Tile:
     """A tile of a kernel: the kernel's name among the plan's items, query rows, keys that a range is a
-    multiple of (one number for all tiles of a kernel), blocks that fill the device."""
+    multiple of (one number for all tiles of a kernel), blocks that the device holds at once; ``places``:
+    partial results that a range leaves."""
     name: str
     rows: int
     unit: int
     blocks: int
+    places: int = 1
+
+
+def choose_range(lengths: np.ndarray, copies: np.ndarray, unit: int, blocks: int) -> int:
+    """How long the ranges are that ``lengths`` are cut into, a multiple of ``unit``: range r of length i
+    is the work of ``copies[i]`` blocks.  Of all numbers of rounds of ``blocks`` blocks the one that is
+    done first, a block costing its keys and as much as ``OVERHEAD`` keys besides."""
+    longest = int(lengths.max(initial=0))
+    whole = -(-longest // unit) * unit
+    best = None
+    count = lambda each: int((-(-lengths // each) * copies).sum())
+    least = -(-count(max(whole, unit)) // blocks)
+    for rounds in range(max(least, 1), max(least, 1) + 4):
+        low, high = 1, max(whole // unit, 1)              # the shortest that needs no more rounds
+        while low < high:
+            mid = (low + high) // 2
+            if count(mid * unit) <= rounds * blocks:
+                high = mid
+            else:
+                low = mid + 1
+        cost = rounds * (low * unit + OVERHEAD)
+        if best is None or cost < best[0]:
+            best = (cost, low * unit)
+    return best[1]
+
+
+OVERHEAD = 256
 
 
 def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, prefix_tile,
@@ -64,23 +92,22 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
     many ranges they are cut into goes by it, not which keys are seen)."""
     qlen = np.asarray(seq_qlen, dtype=np.int64).reshape(-1)
     sizes = np.asarray(group_sizes, dtype=np.int64).reshape(-1)
-    prefix = np.asarray(prefix_lens, dtype=np.int64).reshape(-1)
+    shared = np.asarray(prefix_lens, dtype=np.int64).reshape(-1)
     _need(bool((qlen >= 0).all()), "shared prefix: a request brings no fewer than 0 tokens")
-    _need(len(sizes) == len(prefix) and bool((sizes > 0).all()) and int(sizes.sum()) == len(qlen),
+    _need(len(sizes) == len(shared) and bool((sizes > 0).all()) and int(sizes.sum()) == len(qlen),
           "shared prefix: group sizes are positive and add up to the requests, with a prefix each")
-    _need(bool((prefix >= 0).all()) and int(tail) >= 0, "shared prefix: lengths are not negative")
+    _need(bool((shared >= 0).all()) and int(tail) >= 0, "shared prefix: lengths are not negative")
     total = int(qlen.sum())
-    _need(total * group < 1 << 28 and int(prefix.max(initial=0)) < 1 << 31,
+    _need(total * group < 1 << 28 and int(shared.max(initial=0)) < 1 << 31,
           "shared prefix: the step has too many rows or keys")
     tok0 = np.cumsum(qlen) - qlen
     first = np.cumsum(sizes) - sizes
-    group_tokens = np.add.reduceat(qlen, first) if len(sizes) else np.zeros(0, dtype=np.int64)
-    group_tok0 = tok0[first] if len(sizes) else np.zeros(0, dtype=np.int64)
+    live = np.add.reduceat((qlen > 0).astype(np.int64), first) if len(sizes) else sizes
     # a prefix that only one request's rows read is no different from its own keys
-    members = np.add.reduceat((qlen > 0).astype(np.int64), first) if len(sizes) else sizes
-    prefix = np.where(members > 1, prefix, 0)
+    prefix = np.where(live > 1, shared, 0)
+    rows = (np.add.reduceat(qlen, first) if len(sizes) else sizes) * group
     seqs = np.zeros((len(qlen), 8), dtype=np.int64)
-    seqs[:, 0], seqs[:, 1] = tok0, np.repeat(group_tok0, sizes)
+    seqs[:, 0], seqs[:, 1] = tok0, np.repeat(tok0[first], sizes)
     items: dict[str, list] = {}
     shapes: dict[str, tuple] = {}
     base = 0
@@ -89,63 +116,60 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
         items.setdefault(t.name, []).append(part)
         shapes[t.name] = (max(t.rows, shapes.get(t.name, (0, 0))[0]), t.unit)
 
-    # shared keys: ranges of one length for all groups, so long that the blocks fill the device once
-    tiles = [prefix_tile(int(t) * group) for t in group_tokens]
-    work: dict[str, int] = {}
-    for t, p, n in zip(tiles, prefix, group_tokens):
-        work[t.name] = work.get(t.name, 0) + -(-int(n) * group // t.rows) * int(p) * kv_heads
-    for g, (t, p, n) in enumerate(zip(tiles, prefix, group_tokens)):
-        rows, p = int(n) * group, int(p)
-        if p == 0 or rows == 0:
-            continue
-        each = -(-max(work[t.name] // t.blocks, t.unit) // t.unit) * t.unit
-        chunks = -(-p // each)
-        each = -(-(-(-p // chunks)) // t.unit) * t.unit
-        chunks = -(-p // each)
-        count = -(-rows // t.rows)
-        tile, chunk = np.divmod(np.arange(count * chunks), chunks)
-        part = np.zeros((count * chunks, 8), dtype=np.int64)
-        part[:, 0], part[:, 2] = group_tok0[g], tile * t.rows
-        part[:, 1] = np.minimum(t.rows, rows - part[:, 2])
-        part[:, 3], part[:, 4] = first[g], chunk * each
-        part[:, 5] = np.minimum(p, (chunk + 1) * each)
-        part[:, 7] = base + (tile * chunks + chunk) * t.rows
-        # a range after the other, its tiles side by side: they read the same keys
-        add(t, part[np.argsort(chunk, kind="stable")])
-        members_of = slice(int(first[g]), int(first[g] + sizes[g]))
-        seqs[members_of, 2], seqs[members_of, 3], seqs[members_of, 4] = base, chunks, t.rows
-        base += count * chunks * t.rows
+    # shared keys
+    by_name: dict[str, list] = {}
+    for g in np.nonzero((prefix > 0) & (rows > 0))[0]:
+        t = prefix_tile(int(rows[g]))
+        by_name.setdefault(t.name, []).append((int(g), t))
+    for members in by_name.values():
+        lengths = prefix[[g for g, _ in members]]
+        copies = np.asarray([-(-int(rows[g]) // t.rows) * kv_heads for g, t in members])
+        each = choose_range(lengths, copies, members[0][1].unit, members[0][1].blocks)
+        for g, t in members:
+            p, n = int(prefix[g]), int(rows[g])
+            chunks, count = -(-p // each), -(-n // t.rows)
+            size = -(-(-(-p // chunks)) // t.unit) * t.unit          # ranges of about one length
+            chunks = -(-p // size)
+            tile, chunk = np.divmod(np.arange(count * chunks), chunks)
+            part = np.zeros((count * chunks, 8), dtype=np.int64)
+            part[:, 0], part[:, 2] = tok0[first[g]], tile * t.rows
+            part[:, 1] = np.minimum(t.rows, n - part[:, 2])
+            part[:, 3], part[:, 4] = first[g], chunk * size
+            part[:, 5] = np.minimum(p, (chunk + 1) * size)
+            part[:, 6] = t.places - 1
+            part[:, 7] = base + (tile * chunks + chunk) * t.rows * t.places
+            # a range after the other, its tiles side by side: they read the same keys
+            add(t, part[np.argsort(chunk, kind="stable")])
+            s = slice(int(first[g]), int(first[g] + sizes[g]))
+            seqs[s, 2], seqs[s, 3], seqs[s, 4] = base, chunks * t.places, t.rows
+            base += count * chunks * t.rows * t.places
 
-    # each request's own keys
-    live = np.nonzero(qlen > 0)[0]
-    if len(live):
-        by_tile: dict[Tile, list] = {}
-        for s in live:
-            by_tile.setdefault(own_tile(int(qlen[s]) * group), []).append(int(s))
-        for t, members_of in by_tile.items():
-            s = np.asarray(members_of)
-            rows = qlen[s] * group
-            count = -(-rows // t.rows)
-            own = np.maximum(int(tail), qlen[s]) + np.where(np.repeat(prefix, sizes)[s] > 0, 0,
-                                                            np.repeat(np.asarray(
-                                                                prefix_lens, dtype=np.int64), sizes)[s])
-            need = int((count * own).sum()) * kv_heads
-            each = max(-(-need // t.blocks), t.unit)
-            splits = np.clip(-(-own // each), 1, MAX_SPLITS)
-            n = count * splits
-            owner = np.repeat(np.arange(len(s)), n)
-            at = np.arange(int(n.sum())) - np.repeat(np.cumsum(n) - n, n)
-            tile, split = at // splits[owner], at % splits[owner]
-            start = base + np.cumsum(n * t.rows) - n * t.rows
-            part = np.zeros((len(owner), 8), dtype=np.int64)
-            part[:, 0], part[:, 2] = tok0[s[owner]], tile * t.rows
-            part[:, 1] = np.minimum(t.rows, rows[owner] - part[:, 2])
-            part[:, 3], part[:, 4], part[:, 5] = s[owner], np.repeat(prefix, sizes)[s[owner]], -1
-            part[:, 6] = split | splits[owner] << 16
-            part[:, 7] = start[owner] + (tile * splits[owner] + split) * t.rows
-            add(t, part)
-            seqs[s, 5], seqs[s, 6], seqs[s, 7] = start, splits, t.rows
-            base += int((n * t.rows).sum())
+    # each request's own keys, behind its prefix
+    start = np.repeat(prefix, sizes)
+    own = np.maximum(int(tail), qlen) + np.where(start > 0, 0, np.repeat(shared, sizes))
+    by_tile: dict[Tile, list] = {}
+    for s in np.nonzero(qlen > 0)[0]:
+        by_tile.setdefault(own_tile(int(qlen[s]) * group), []).append(int(s))
+    for t, members in by_tile.items():
+        s = np.asarray(members)
+        n = qlen[s] * group
+        count = -(-n // t.rows)
+        each = choose_range(own[s], count * kv_heads, t.unit, t.blocks)
+        splits = np.clip(-(-own[s] // each), 1, MAX_SPLITS)
+        pieces = count * splits
+        owner = np.repeat(np.arange(len(s)), pieces)
+        at = np.arange(len(owner)) - np.repeat(np.cumsum(pieces) - pieces, pieces)
+        tile, split = at // splits[owner], at % splits[owner]
+        begin = base + np.cumsum(pieces * t.rows) - pieces * t.rows
+        part = np.zeros((len(owner), 8), dtype=np.int64)
+        part[:, 0], part[:, 2] = tok0[s[owner]], tile * t.rows
+        part[:, 1] = np.minimum(t.rows, n[owner] - part[:, 2])
+        part[:, 3], part[:, 4], part[:, 5] = s[owner], start[s[owner]], -1
+        part[:, 6] = split | splits[owner] << 16
+        part[:, 7] = begin[owner] + (tile * splits[owner] + split) * t.rows
+        add(t, part)
+        seqs[s, 5], seqs[s, 6], seqs[s, 7] = begin, splits, t.rows
+        base += int((pieces * t.rows).sum())
     _need(base < 1 << 31, "shared prefix: too many partial results")
     return SharedPlan({name: np.concatenate(parts) for name, parts in items.items()}, shapes, seqs,
                       np.repeat(np.arange(len(qlen)), qlen), base, total)
@@ -168,6 +192,8 @@ class SharedPrefixAttention:
         self.scale, self.group = float(scale), heads // kv_heads
         self.tensor_cores = uses_tensor_cores(dtype, head_dim)
         self.mma_module = ("shared_prefix_mma", (f"HEAD_DIM={head_dim}",))
+        self.tcgen05_module = (("shared_prefix_tcgen05", (f"HEAD_DIM={head_dim}",))
+                               if self.tensor_cores and head_dim in (64, 128) else None)
         self._device = None if device is None else torch.device(device)
         self._sms: "int | None" = None
 
@@ -181,13 +207,22 @@ class SharedPrefixAttention:
     def tiles(self) -> "tuple":
         """(rows of a group -> ``Tile``, rows of a request -> ``Tile``)."""
         sms = self._sm_count()
-        if self.tensor_cores:
-            lib = library.load(*self.mma_module)
-            most, blocks = lib.de_shared_mma_rows(), lib.de_shared_mma_blocks_per_sm() * sms
-            tile = lambda rows: Tile("mma", min(most, max(1, -(-rows // 16)) * 16), 64, blocks)
-            return tile, tile
-        plain = Tile("rows", 8, 32, 4 * sms)
-        return (lambda rows: plain), (lambda rows: plain)
+        if not self.tensor_cores:
+            plain = Tile("rows", 8, 32, 4 * sms)
+            return (lambda rows: plain), (lambda rows: plain)
+        lib = library.load(*self.mma_module)
+        most, blocks = lib.de_shared_mma_rows(), lib.de_shared_mma_blocks_per_sm() * sms
+
+        def few(rows: int) -> Tile:
+            return Tile("mma", min(most, -(-rows // 16) * 16), 64, blocks)
+
+        def many(rows: int) -> Tile:
+            if rows <= most or self.tcgen05_module is None:
+                return few(rows)
+            return (Tile("tcgen05", 128, 128, sms, 2) if rows <= 128 else
+                    Tile("tcgen05", 256, 128, sms))
+
+        return many, few
 
     def host_plan(self, seq_qlen, group_sizes, prefix_lens, tail: int = 0) -> SharedPlan:
         prefix_tile, own_tile = self.tiles()
@@ -240,22 +275,29 @@ class SharedPrefixAttention:
         ml = make("shared_prefix.partial_ml", (rows * 2,), torch.float32)
         lib = library.load("shared_prefix")
         tag = _tag(q.dtype)
-        # (rows that are not in 4-byte pieces, pages that are not in 16-byte ones: one by one)
-        aligned = not (q.stride(0) % 2 or q.data_ptr() % 4 or k_pages.data_ptr() % 16
-                       or v_pages.data_ptr() % 16)
+        # what a kernel copies in pieces has to lie so; the next one in this list takes it otherwise
+        pages_fit = not (k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16)
+        aligned = pages_fit and not (q.stride(0) % 2 or q.data_ptr() % 4)
+        wide = pages_fit and not (q.stride(0) % 8 or q.data_ptr() % 16)
+        behind = 0
         for name, items in plan.items.items():
             rows, unit = plan.shapes[name]
             before = (q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
                       block_table.data_ptr(), block_table.stride(0), k_pages.shape[0],
                       seq_slot.data_ptr(), seq_pos0.data_ptr(), items.data_ptr(), items.shape[0])
-            behind = (acc.data_ptr(), ml.data_ptr(), self.heads, self.kv_heads, d, k_pages.shape[2],
-                      self.scale, status.data_ptr(), _stream())
-            if name == "mma" and aligned:
-                _check(library.load(*self.mma_module).de_shared_mma(*before, *behind),
+            after = (acc.data_ptr(), ml.data_ptr(), self.heads, self.kv_heads, d, k_pages.shape[2],
+                     self.scale, status.data_ptr(), _stream())
+            if (name == "tcgen05" and wide and not behind
+                    and (kernel := library.load(*self.tcgen05_module)).de_shared_tcgen05_page_ok(
+                        k_pages.shape[2])):
+                _check(kernel.de_shared_tcgen05(*before, *after), "shared prefix attention (tcgen05)")
+            elif name != "rows" and aligned:
+                _check(library.load(*self.mma_module).de_shared_mma(*before, rows, behind, *after),
                        "shared prefix attention (mma)")
             else:
-                _check(lib.de_shared_rows(tag, *before, rows, unit, *behind),
+                _check(lib.de_shared_rows(tag, *before, rows, unit, behind, *after),
                        "shared prefix attention")
+            behind = 1
         _check(lib.de_shared_merge(tag, out.data_ptr(), out.stride(0), plan.token_seq.data_ptr(),
                                    plan.seqs.data_ptr(), acc.data_ptr(), ml.data_ptr(), tokens,
                                    self.heads, self.kv_heads, d, _stream()), "shared prefix merge")

@@ -12,6 +12,7 @@ TILES = {
     "one": (Tile("rows", 8, 32, 592),) * 2,
     "two": (Tile("wide", 128, 128, 148), Tile("narrow", 16, 64, 592)),
     "few": (Tile("wide", 32, 64, 3), Tile("narrow", 8, 1, 5)),
+    "places": (Tile("wide", 128, 128, 148, 2), Tile("narrow", 16, 64, 592)),
 }
 STEPS = {
     # tokens a request, requests a group, prefix a group, keys of its own before this step's tokens
@@ -38,9 +39,9 @@ def _seen(plan, tiles, group, kv_heads, qlen, sizes, prefix, own):
         t = rows_of[name]
         for it in items.tolist():
             at, n, row0, seq, begin, end, split, base = it
-            assert 0 < n <= t.rows and 0 <= base and base + t.rows <= plan.partial_rows
+            assert 0 < n <= t.rows and 0 <= base and base + t.rows * t.places <= plan.partial_rows
             assert plan.shapes[name] == (t.rows, t.unit)
-            used[base: base + t.rows] += 1
+            used[base: base + t.rows * t.places] += 1
             if end < 0:                               # as range_of in the kernels' header
                 assert at == tok0[seq]
                 stop = max(begin, pos0[seq] + (row0 + n - 1) // group + 1)
@@ -51,6 +52,7 @@ def _seen(plan, tiles, group, kv_heads, qlen, sizes, prefix, own):
             else:
                 assert seq == first[group_of[seq]] and at == tok0[seq]
                 lo, hi = begin, end
+                assert begin < end and begin % t.unit == 0 and split == t.places - 1
             for r in range(n):
                 token = at + (row0 + r) // group
                 limit = hi
@@ -58,6 +60,8 @@ def _seen(plan, tiles, group, kv_heads, qlen, sizes, prefix, own):
                     limit = min(hi, pos0[seq] + (row0 + r) // group + 1)
                 by_row.setdefault((token, (row0 + r) % group), []).append(
                     (lo, max(lo, limit), base + r))
+                if end >= 0 and split:                # the place of the range's other half
+                    by_row[token, (row0 + r) % group].append((lo, lo, base + t.rows + r))
     assert (used == 1).all()
     return by_row, pos0, tok0
 
