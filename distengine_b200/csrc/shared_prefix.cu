@@ -26,6 +26,7 @@ using namespace shared_prefix;
 constexpr int ROWS = 8;               // query rows of a block
 constexpr int KT = 32;                // keys of a tile
 constexpr int THREADS = 128;
+constexpr int MERGE_MOST = 1024;       // partial results of a row
 
 // A block takes eight rows of an item (blockIdx.y: which), a warp two.  Scores: a lane a key;
 // results: a lane every 32nd feature.
@@ -140,32 +141,41 @@ shared_rows_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ 
     if (behind) pdl_wait();
 }
 
-// A warp a (token, query head): the lanes take the partial results' maxima and sums in turn, then
-// all of them the features of one partial result after the other.
-template <typename T>
+// A warp a (token, query head).  The lanes take the partial results' maxima and sums in turn, which
+// gives each its weight; then the weighted results are summed, LANES lanes a result (a lane four
+// features at a time where VEC) and several results at once.
+template <typename T, int LANES, bool VEC>
 __global__ void __launch_bounds__(128)
 shared_merge_kernel(T* __restrict__ out, int out_stride, const int* __restrict__ token_seq,
                     const Joined* __restrict__ seqs, const float* __restrict__ partial_acc,
                     const float2* __restrict__ partial_ml, int tokens, int heads, int kv_heads,
                     int d) {
+    constexpr int AT_ONCE = 32 / LANES, N = VEC ? 4 : 8, DEEP = VEC ? 4 : 1;
+    __shared__ float weight_s[4][MERGE_MOST];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long unit = (long long)blockIdx.x * 4 + warp;
-    pdl_wait();
-    pdl_trigger();
-    if (unit >= (long long)tokens * heads) return;
-    const int token = (int)(unit / heads), h = (int)(unit % heads);
+    const bool there = unit < (long long)tokens * heads;
+    const int token = there ? (int)(unit / heads) : 0, h = (int)(unit % heads);
     const int g = heads / kv_heads, hk = h / g;
     const Joined s = seqs[token_seq[token]];
+    // the results of a row lie a tile's rows apart: the prefix's, then its own keys'
+    const int row_p = (token - s.group_tok0) * g + h % g, row_o = (token - s.tok0) * g + h % g;
     const int parts = s.prefix_chunks + s.own_chunks;
+    size_t at_p = 0, at_o = 0;
+    if (s.prefix_chunks)
+        at_p = (size_t)(s.prefix_base + row_p / s.prefix_rows * s.prefix_chunks * s.prefix_rows +
+                        row_p % s.prefix_rows) * kv_heads + hk;
+    if (s.own_chunks)
+        at_o = (size_t)(s.own_base + row_o / s.own_rows * s.own_chunks * s.own_rows +
+                        row_o % s.own_rows) * kv_heads + hk;
     auto place = [&](int c) {
-        const bool shared = c < s.prefix_chunks;
-        const int row = (token - (shared ? s.group_tok0 : s.tok0)) * g + h % g;
-        const int tile = shared ? s.prefix_rows : s.own_rows;
-        const int chunks = shared ? s.prefix_chunks : s.own_chunks;
-        const int base = shared ? s.prefix_base : s.own_base;
-        const int chunk = shared ? c : c - s.prefix_chunks;
-        return (size_t)(base + (row / tile * chunks + chunk) * tile + row % tile) * kv_heads + hk;
+        return c < s.prefix_chunks
+                   ? at_p + (size_t)c * s.prefix_rows * kv_heads
+                   : at_o + (size_t)(c - s.prefix_chunks) * s.own_rows * kv_heads;
     };
+    pdl_wait();
+    pdl_trigger();
+    if (!there) return;
     float top = -INFINITY;
     for (int c = lane; c < parts; c += 32) top = fmaxf(top, partial_ml[place(c)].x);
     top = warp_max(top);
@@ -173,29 +183,70 @@ shared_merge_kernel(T* __restrict__ out, int out_stride, const int* __restrict__
     float total = 0.0f;
     for (int c = lane; c < parts; c += 32) {
         const float2 ml = partial_ml[place(c)];
-        total += exp2f(ml.x - top) * ml.y;
+        // (a range without a key has left no result; one of NaN scores only has a sum that is NaN)
+        const bool empty = ml.x == -INFINITY && ml.y == 0.0f;
+        const float w = empty ? 0.0f : exp2f(ml.x - top);
+        total += empty ? 0.0f : w * ml.y;
+        weight_s[warp][c] = empty ? -1.0f : w;
     }
     total = warp_sum(total);
-    float acc[8];
+    __syncwarp();
+    const int sub = lane % LANES, which = lane / LANES;
+    float acc[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
-    for (int c = 0; c < parts; ++c) {
-        const size_t at = place(c);
-        const float2 ml = partial_ml[at];
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;             // no key in this range
-        const float w = exp2f(ml.x - top);
+    for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+    for (int c0 = which; c0 < parts; c0 += AT_ONCE * DEEP) {
+        if constexpr (VEC) {
+            float4 v[DEEP];
+            float w[DEEP];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int f = lane + 32 * i;
-            if (f < d) acc[i] = fmaf(w, partial_acc[at * d + f], acc[i]);
+            for (int k = 0; k < DEEP; ++k) {
+                const int c = c0 + k * AT_ONCE;
+                w[k] = c < parts ? weight_s[warp][c] : -1.0f;
+                v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (w[k] >= 0.0f || w[k] != w[k])
+                    v[k] = *reinterpret_cast<const float4*>(partial_acc + place(c) * d + 4 * sub);
+            }
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k) {
+                if (w[k] == -1.0f) continue;
+                acc[0] = fmaf(w[k], v[k].x, acc[0]);
+                acc[1] = fmaf(w[k], v[k].y, acc[1]);
+                acc[2] = fmaf(w[k], v[k].z, acc[2]);
+                acc[3] = fmaf(w[k], v[k].w, acc[3]);
+            }
+        } else {
+            const float w = weight_s[warp][c0];
+            if (w == -1.0f) continue;
+            const size_t at = place(c0);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (sub + LANES * i < d) acc[i] = fmaf(w, partial_acc[at * d + sub + LANES * i], acc[i]);
         }
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int f = lane + 32 * i;
-        if (f < d) out[(size_t)token * out_stride + h * d + f] = from_float<T>(acc[i] * inv);
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int o = LANES; o < 32; o <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    T* dst = out + (size_t)token * out_stride + h * d;
+    if (which != 0) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int f = VEC ? 4 * sub + i : sub + LANES * i;
+        if (f < d) dst[f] = from_float<T>(acc[i] * inv);
     }
+}
+
+template <typename T>
+int merge_of(void* out, int out_stride, const int* token_seq, const int* seqs, const float* partial_acc,
+             const float* partial_ml, int tokens, int heads, int kv_heads, int d, cudaStream_t stream) {
+    const auto kernel = d == 128  ? shared_merge_kernel<T, 32, true>
+                        : d == 64 ? shared_merge_kernel<T, 16, true>
+                                  : shared_merge_kernel<T, 32, false>;
+    return de_launch(kernel, dim3((unsigned)(((long long)tokens * heads + 3) / 4)), dim3(128), 0, stream,
+                     (T*)out, out_stride, token_seq, (const Joined*)seqs, partial_acc,
+                     (const float2*)partial_ml, tokens, heads, kv_heads, d);
 }
 
 template <typename T>
@@ -237,17 +288,14 @@ DE_EXPORT int de_shared_rows(int dtype, const void* q, int q_stride, const void*
              (cudaStream_t)stream);
 }
 
+// No row has more than de_shared_merge_most() partial results.
+DE_EXPORT int de_shared_merge_most() { return MERGE_MOST; }
 DE_EXPORT int de_shared_merge(int dtype, void* out, int out_stride, const int* token_seq,
                               const int* seqs, const float* partial_acc, const float* partial_ml,
                               int tokens, int heads, int kv_heads, int head_dim, void* stream) {
     if (tokens <= 0) return 0;
     if (head_dim < 2 || head_dim > 256 || head_dim % 2 || kv_heads < 1 || heads % kv_heads) return -2;
-    const dim3 grid((unsigned)(((long long)tokens * heads + 3) / 4)), block(128);
-    if (dtype == DE_F32)
-        return de_launch(shared_merge_kernel<float>, grid, block, 0, (cudaStream_t)stream, (float*)out,
-                         out_stride, token_seq, (const Joined*)seqs, partial_acc,
-                         (const float2*)partial_ml, tokens, heads, kv_heads, head_dim);
-    return de_launch(shared_merge_kernel<__nv_bfloat16>, grid, block, 0, (cudaStream_t)stream,
-                     (__nv_bfloat16*)out, out_stride, token_seq, (const Joined*)seqs, partial_acc,
-                     (const float2*)partial_ml, tokens, heads, kv_heads, head_dim);
+    const auto f = dtype == DE_F32 ? merge_of<float> : merge_of<__nv_bfloat16>;
+    return f(out, out_stride, token_seq, seqs, partial_acc, partial_ml, tokens, heads, kv_heads, head_dim,
+             (cudaStream_t)stream);
 }

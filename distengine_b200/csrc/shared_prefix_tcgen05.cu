@@ -7,12 +7,12 @@
 //   * up to 128 rows: both pipelines have the same rows and take the key tiles in turn, each for a
 //     partial result of its own, so that one's exponentials run beside the other's products here too.
 // Warps:
-//   * warps 0-3 and 4-7 are the pipelines' softmax threads, one thread a row (= a lane of tensor
-//     memory): a tile's 128 scores into registers, exponentials in float32, weights as bfloat16 back
-//     into tensor memory as the A operand of the second product;
-//   * warp 8, one thread, issues s = q k^T (operands in shared memory) and o += p v (p in tensor
-//     memory, v MN-major straight from the pages) for whichever pipeline is ready;
-//   * warp 9 fetches: a ring of buffers of 128 keys or 128 values, one TMA box a page and 64 features.
+//   * warps 0-7 and 8-15 are the pipelines' softmax threads, two threads a row (= a lane of tensor
+//     memory), each 32 keys of either half of a tile: 64 scores into registers, exponentials in float32, weights as
+//     bfloat16 back into tensor memory as the A operand of the second product;
+//   * warps 16 and 17, one thread each, issue a pipeline's s = q k^T (operands in shared memory) and
+//     o += p v (p in tensor memory, v MN-major straight from the pages);
+//   * warp 18 fetches: a ring of buffers of 128 keys or 128 values, one TMA box a page and 64 features.
 // A row's exponentials refer to a maximum that is raised, and o rescaled, only when a score has grown by
 // more than 2^8 beyond it.
 //
@@ -48,9 +48,9 @@ constexpr int KT = 128;                       // keys of a tile
 constexpr int SUB = 128 * 128;                // bytes of a sub-tile: 128 rows of 64 features
 constexpr int BUFFER = KS * SUB;              // 128 keys, or their values
 constexpr int BUFFERS = D == 64 ? 10 : 5;     // what shared memory has room for beside q
-constexpr int THREADS = 10 * 32;
-constexpr int MMA_WARP = 8, COPY_WARP = 9;
-constexpr int SMEM = 2 * BUFFER + BUFFERS * BUFFER + 512;
+constexpr int SOFTMAX_WARPS = 16, MMA_WARP = 16, COPY_WARP = 18;
+constexpr int THREADS = 19 * 32;
+constexpr int SMEM = 2 * BUFFER + BUFFERS * BUFFER + 512 + 2 * 2 * LANES * 4;
 constexpr int COLUMNS = 512;
 // columns of tensor memory: scores of pipeline x at 128 x; results at 256 + D x; weights (64 columns) over
 // the scores at head size 128, where there is no other room, and at 384 + 64 x at head size 64
@@ -58,39 +58,79 @@ constexpr bool OVER = D == 128;
 constexpr int O_COL = 256;
 __device__ __forceinline__ unsigned p_col(int x) { return OVER ? 128u * x : 384u + 64u * x; }
 constexpr float RAISE = 8.0f;
+constexpr int ROW_BYTES = D * 4 + 16;         // of a row's results in shared memory: no two lanes on one bank
+static_assert(2 * LANES * ROW_BYTES <= BUFFERS * BUFFER, "the ring holds the results");
 
-__device__ __forceinline__ bool mbar_test(void* bar, unsigned parity) {
-    unsigned done;
+// Bounded wait for the phase with the given parity, as tc5::mbar_wait, but a thread sleeps for up to
+// some microseconds a look: 16 warps that look as often as they can take the issue slots of those
+// that have work.
+__device__ __forceinline__ bool wait(void* bar, unsigned parity, int* status) {
+    const unsigned addr = smem_u32(bar);
+    for (unsigned spins = 0; spins < SPIN_LIMIT / 16; ++spins) {
+        unsigned done;
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(done) : "r"(addr), "r"(parity), "r"(4000u) : "memory");
+        if (done) return true;
+    }
+    atomicExch(status, 3);
+    return false;
+}
+// The products and their commits are issued by a whole warp, of which one elected thread (the same every
+// time) takes effect: so the operands are known to be the same in all lanes.  Behind a branch on the lane
+// an instruction takes 160 cycles to issue, eight of 128 x 128 x 16 1,307 instead of their 514.
+__device__ __forceinline__ void umma(unsigned d, unsigned long long a_desc, unsigned long long b_desc,
+                                     unsigned idesc, bool accumulate) {
     asm volatile(
         "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
+        ".reg .pred p, e;\n"
+        "elect.sync _|e, 0xffffffff;\n"
+        "setp.ne.u32 p, %4, 0;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
         "}\n"
-        : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    return done != 0;
+        ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((unsigned)accumulate) : "memory");
 }
 __device__ __forceinline__ void umma_a_tmem(unsigned d, unsigned a, unsigned long long b_desc,
                                             unsigned idesc, bool accumulate) {
     asm volatile(
         "{\n"
-        ".reg .pred p;\n"
+        ".reg .pred p, e;\n"
+        "elect.sync _|e, 0xffffffff;\n"
         "setp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
         "}\n"
         ::"r"(d), "r"(a), "l"(b_desc), "r"(idesc), "r"((unsigned)accumulate) : "memory");
 }
-__device__ __forceinline__ void tmem_store_32cols(unsigned taddr, const unsigned (&r)[32]) {
+__device__ __forceinline__ void commit(void* bar) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n"
+        "{\n"
+        ".reg .pred e;\n"
+        "elect.sync _|e, 0xffffffff;\n"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+        "}\n"
+        ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_store_16cols(unsigned taddr, const unsigned (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
           "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-          "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-          "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-          "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+          "r"(r[14]), "r"(r[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_load_16cols(unsigned taddr, unsigned (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_stores() {
     asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
@@ -106,10 +146,51 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
     return y;
 }
+// pairs of float32 numbers, for the instructions that take two at once
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float a, float b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void untwo(Two v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ Two fma_two(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ Two add_two(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max_three(float a, unsigned b, unsigned c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+    return r;
+}
 __device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool pred) {
     const int bytes = pred ? 16 : 0;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem),
                  "r"(bytes));
+}
+// The two warps that share their rows: whether a thread of either says so, and their barrier.
+__device__ __forceinline__ bool any_of_pair(int barrier, bool mine) {
+    unsigned any;
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.u32 p, %1, 0;\n"
+        "barrier.cta.red.or.pred q, %2, 64, p;\n"
+        "selp.u32 %0, 1, 0, q;\n"
+        "}\n"
+        : "=r"(any) : "r"((unsigned)mine), "r"(barrier) : "memory");
+    return any != 0;
+}
+__device__ __forceinline__ void sync_pair(int barrier) {
+    asm volatile("barrier.cta.sync %0, 64;\n" ::"r"(barrier) : "memory");
 }
 // v as the second operand: MN-major, 128-byte swizzle, from 64 features to the next 64 a sub-tile
 __device__ __forceinline__ unsigned long long value_desc(const void* tile) {
@@ -119,6 +200,10 @@ __device__ __forceinline__ unsigned long long value_desc(const void* tile) {
 }
 constexpr unsigned DESC_S = instr_desc(128, KT);
 constexpr unsigned DESC_O = instr_desc(128, D) | 1u << 16;
+
+template <bool B> struct Truth {
+    static constexpr bool value = B;
+};
 
 __global__ void __launch_bounds__(THREADS, 1)
 shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
@@ -135,12 +220,14 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
     unsigned long long* full = bars;                      // [BUFFERS] the pages have landed
     unsigned long long* empty = bars + BUFFERS;           // [BUFFERS] the products that read it are done
     unsigned long long* s_done = bars + 2 * BUFFERS;      // [2] scores are complete
-    unsigned long long* p_ready = s_done + 2;             // [2] weights are written (128 arrivals)
+    unsigned long long* p_ready = s_done + 2;             // [2] weights are written (256 arrivals)
     unsigned long long* o_done = s_done + 4;              // [2] weights times values is complete
-    unsigned long long* s_free = s_done + 6;              // [2] scores are in registers (128 arrivals)
-    unsigned long long* drained = s_done + 8;             // everything issued is complete, after a failed wait
-    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(s_done + 9);
-    int& missing_s = *reinterpret_cast<int*>(s_done + 10);
+    unsigned long long* s_free = s_done + 6;              // [2] scores are in registers (256 arrivals)
+    unsigned long long* drained = s_done + 8;             // [2] what is issued is complete, after a failed wait
+    unsigned long long* p_half = s_done + 10;             // [2] those of the first 64 keys are
+    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(s_done + 12);
+    int& missing_s = *reinterpret_cast<int*>(s_done + 13);
+    float* exchange = reinterpret_cast<float*>(ring + BUFFERS * BUFFER + 512);   // [pipeline][half][row]
 
     const Item it = items[blockIdx.x / kv_heads];
     const int hk = blockIdx.x % kv_heads, g = heads / kv_heads;
@@ -156,16 +243,18 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
 
     if (tid == 0) {
         missing_s = 0;
-        mbar_init(drained, 1);
+        mbar_init(&drained[0], 1);
+        mbar_init(&drained[1], 1);
         for (int i = 0; i < BUFFERS; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            mbar_init(&empty[i], !turns && it.count > LANES ? 2 : 1);      // pipelines that read it
         }
         for (int x = 0; x < 2; ++x) {
             mbar_init(&s_done[x], 1);
-            mbar_init(&p_ready[x], LANES);
+            mbar_init(&p_ready[x], 2 * LANES);
+            mbar_init(&p_half[x], 2 * LANES);
             mbar_init(&o_done[x], 1);
-            mbar_init(&s_free[x], LANES);
+            mbar_init(&s_free[x], 2 * LANES);
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -193,17 +282,20 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             missing_s = 1;
         }
     }
-    const int x = warp < 8 ? warp >> 2 : 0;               // pipeline
+    const int x = warp < SOFTMAX_WARPS ? warp >> 3 : 0;   // pipeline
+    const int half = warp >> 2 & 1;                       // of a tile's keys, of a row's features
     const int rowi = (warp & 3) * 32 + lane;              // row of the pipeline
     const int row = turns ? rowi : x * LANES + rowi;      // of the item
-    const bool live = warp < 8 && row < it.count;
-    if (warp < 8) {                   // q in the operand layout: 16-byte piece c at place c xor row % 8
+    const bool live = warp < SOFTMAX_WARPS && row < it.count;
+    if (warp < SOFTMAX_WARPS) {                   // q in the operand layout: 16-byte piece c at place c xor row % 8
         const int r = it.row0 + (live ? row : 0);
         const __nv_bfloat16* src = q + (size_t)(it.tok0 + r / g) * q_stride + (hk * g + r % g) * D;
         unsigned char* dst = q_s + x * BUFFER + rowi * 128;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c)
+        for (int e = 0; e < D / 16; ++e) {
+            const int c = half * (D / 16) + e;
             cp_async16(dst + (c >> 3) * SUB + (((c & 7) ^ (rowi & 7)) << 4), src + c * 8, live);
+        }
         asm volatile("cp.async.commit_group;\n" ::);
         asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     }
@@ -229,7 +321,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
                 const int unit = 2 * t + v, b = unit % BUFFERS;
-                if (unit >= BUFFERS && ok) ok = mbar_wait(&empty[b], (unit / BUFFERS - 1) & 1, status);
+                if (unit >= BUFFERS && ok) ok = wait(&empty[b], (unit / BUFFERS - 1) & 1, status);
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 if (!ok) break;
                 if (lane == 0) mbar_expect_tx(&full[b], bytes);
@@ -245,90 +337,79 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         }
         if (!ok)                      // what is on its way lands before the block ends
             for (int u = max(0, issued - BUFFERS); u < issued; ++u)
-                mbar_wait(&full[u % BUFFERS], (u / BUFFERS) & 1, status);
-    } else if (warp == MMA_WARP) {
+                wait(&full[u % BUFFERS], (u / BUFFERS) & 1, status);
+    } else if (warp >= MMA_WARP) {
         // ------------------------------------------------------------------ tensor cores
-        if (lane == 0) {
-            int s_next[2] = {0, 0}, o_next[2] = {0, 0};   // products of each pipeline issued so far
-            int k_freed = 0, v_freed = 0;                 // tiles whose buffers are handed back
-            unsigned idle = 0;
-            while (ok && (o_next[0] < n_of[0] || o_next[1] < n_of[1])) {
-                bool progress = false;
+        const int i = __shfl_sync(0xffffffffu, warp - MMA_WARP, 0);
+        const int n = i ? n_of[1] : n_of[0];
+        // (all lanes wait, and go on together)
+        auto passed = [&](void* bar, unsigned parity) {
+            if (ok) ok = wait(bar, parity, status);
+            ok = __all_sync(0xffffffffu, ok);
+            after_sync();
+            return ok;
+        };
+        // (a buffer's wait first: it is over long before the other one nearly always)
+        auto scores = [&](int j, void* bar, unsigned parity) {
+            const int unit = 2 * tile_of(i, j), b = unit % BUFFERS;
+            if (ok) ok = wait(&full[b], (unit / BUFFERS) & 1, status);
+            if (!passed(bar, parity)) return;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (o_next[i] < s_next[i]) {
-                        const int j = o_next[i], unit = 2 * tile_of(i, j) + 1, b = unit % BUFFERS;
-                        if (mbar_test(&p_ready[i], j & 1) && mbar_test(&full[b], (unit / BUFFERS) & 1)) {
-                            after_sync();
-                            const unsigned long long vb = value_desc(ring + b * BUFFER);
+            for (int sub = 0; sub < KS; ++sub) {
+                const unsigned long long a = smem_desc(q_s + i * BUFFER + sub * SUB);
+                const unsigned long long kb = smem_desc(ring + b * BUFFER + sub * SUB);
 #pragma unroll
-                            for (int k = 0; k < KT / 16; ++k)
-                                umma_a_tmem(tmem + O_COL + D * i, tmem + p_col(i) + 8 * k,
-                                            vb + (unsigned long long)(k * 2048 >> 4), DESC_O,
-                                            j > 0 || k > 0);
-                            umma_commit(&o_done[i]);
-                            ++o_next[i];
-                            progress = true;
-                            if (turns) umma_commit(&empty[b]);
-                        }
-                    }
-                    if (s_next[i] < n_of[i]) {
-                        const int j = s_next[i], unit = 2 * tile_of(i, j), b = unit % BUFFERS;
-                        // the columns are free: the last weights are multiplied (where they lie over the
-                        // scores), or the last scores in registers
-                        const bool free = j == 0 || (OVER ? o_next[i] == j && mbar_test(&o_done[i], (j - 1) & 1)
-                                                          : mbar_test(&s_free[i], (j - 1) & 1));
-                        if (free && mbar_test(&full[b], (unit / BUFFERS) & 1)) {
-                            after_sync();
-#pragma unroll
-                            for (int sub = 0; sub < KS; ++sub) {
-                                const unsigned long long a = smem_desc(q_s + i * BUFFER + sub * SUB);
-                                const unsigned long long kb = smem_desc(ring + b * BUFFER + sub * SUB);
-#pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    umma_bf16(tmem + 128 * i, a + 2 * k, kb + 2 * k, DESC_S,
-                                              sub > 0 || k > 0);
-                            }
-                            umma_commit(&s_done[i]);
-                            ++s_next[i];
-                            progress = true;
-                            if (turns) umma_commit(&empty[b]);
-                        }
-                    }
-                }
-                if (!turns) {                             // a buffer goes back when both have read it
-                    while (k_freed < s_next[0] && (n_of[1] == 0 || k_freed < s_next[1]))
-                        umma_commit(&empty[2 * k_freed++ % BUFFERS]);
-                    while (v_freed < o_next[0] && (n_of[1] == 0 || v_freed < o_next[1]))
-                        umma_commit(&empty[(2 * v_freed++ + 1) % BUFFERS]);
-                }
-                if (progress) {
-                    idle = 0;
-                } else if (++idle > SPIN_LIMIT) {
-                    atomicExch(status, 3);
-                    ok = false;
-                }
+                for (int k = 0; k < 4; ++k)
+                    umma(tmem + 128 * i, a + 2 * k, kb + 2 * k, DESC_S, sub > 0 || k > 0);
             }
-            if (!ok) {                // what is issued ends before the tensor memory is freed
-                umma_commit(drained);
-                mbar_wait(drained, 0, status);
-            }
+            commit(&s_done[i]);
+            commit(&empty[b]);
+        };
+        if (n > 0) scores(0, &full[2 * tile_of(i, 0)], 0);
+        for (int j = 0; j < n && ok; ++j) {
+            if (!OVER && j + 1 < n) scores(j + 1, &s_free[i], j & 1);     // once these are in registers
+            const int unit = 2 * tile_of(i, j) + 1, b = unit % BUFFERS;
+            const unsigned long long vb = value_desc(ring + b * BUFFER);
+            if (ok) ok = wait(&full[b], (unit / BUFFERS) & 1, status);
+            if (!passed(&p_half[i], j & 1)) break;
+#pragma unroll
+            for (int k = 0; k < KT / 32; ++k)
+                umma_a_tmem(tmem + O_COL + D * i, tmem + p_col(i) + 8 * k,
+                            vb + (unsigned long long)(k * 2048 >> 4), DESC_O, j > 0 || k > 0);
+            if (!passed(&p_ready[i], j & 1)) break;
+#pragma unroll
+            for (int k = KT / 32; k < KT / 16; ++k)
+                umma_a_tmem(tmem + O_COL + D * i, tmem + p_col(i) + 8 * k,
+                            vb + (unsigned long long)(k * 2048 >> 4), DESC_O, true);
+            commit(&o_done[i]);
+            commit(&empty[b]);
+            if (OVER && j + 1 < n) scores(j + 1, &o_done[i], j & 1);      // the weights lie where they will
+        }
+        if (!ok) {                    // what is issued ends before the tensor memory is freed
+            commit(&drained[i]);
+            wait(&drained[i], 0, status);
         }
         __syncwarp();
     } else {
         // ------------------------------------------------------------------ softmax
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-        const unsigned s_addr = tmem + 128 * x + lanes, p_addr = tmem + p_col(x) + lanes;
-        const unsigned o_addr = tmem + O_COL + D * x + lanes;
+        const unsigned s_addr = tmem + 128 * x + 32 * half + lanes;
+        const unsigned p_addr = tmem + p_col(x) + 16 * half + lanes;
+        const unsigned o_addr = tmem + O_COL + D * x + D / 2 * half + lanes;
+        const int pair = 1 + 4 * x + (warp & 3);          // the barrier of the two warps of the same rows
+        float* mine = exchange + (2 * x + half) * LANES + rowi;
+        float* other = exchange + (2 * x + (half ^ 1)) * LANES + rowi;
         const float sl = scale * 1.4426950408889634f;
         float m_ref = -INFINITY, l_run = 0.0f;
-        for (int j = 0; j < n_of[x]; ++j) {
+        // EDGE: a tile in which keys are hidden (a form of its own, so that the others' code is free of it)
+        auto tile = [&](int j, auto edge) {
+            constexpr bool EDGE = decltype(edge)::value;
             const int t = tile_of(x, j), kt = it.begin + t * KT;
-            if (ok) ok = mbar_wait(&s_done[x], j & 1, status);
+            if (ok) ok = wait(&s_done[x], j & 1, status);
             after_sync();
-            unsigned sv[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_load_32cols(s_addr + 32 * c, sv[c]);
+            unsigned sv[2][32];
+            tmem_load_32cols(s_addr, sv[0]);
+            tmem_load_32cols(s_addr + 64, sv[1]);
             tmem_wait_loads();
             if (!OVER) {
                 before_sync();
@@ -336,108 +417,144 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             }
             // keys behind the range, or without a page, are not seen
             unsigned gone = 0;                            // boxes without a page
-            if (missing) {
+            if constexpr (EDGE) {
                 const int key = kt + lane * box;
                 gone = __ballot_sync(0xffffffffu, lane < boxes && key < it.end && page_at(key) < 0);
-            }
-            if (kt + KT > it.end || gone) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 2; ++c) {
+                    const int n = 64 * c + 32 * half + lane;
+                    const unsigned seen =
+                        __ballot_sync(0xffffffffu, kt + n < it.end && !(gone >> (n / box) & 1));
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int n = 32 * c + i;
-                        if (kt + n >= it.end || (gone >> (n / box) & 1)) sv[c][i] = 0xff800000u;
-                    }
+                    for (int i = 0; i < 32; ++i)
+                        if (!(seen >> i & 1)) sv[c][i] = 0xff800000u;
+                }
             }
             float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int i = 0; i < 32; i += 4)
 #pragma unroll
-                for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(sv[c][i]));
+                for (int c = 0; c < 2; ++c) {
+                    m4[c] = max_three(m4[c], sv[c][i], sv[c][i + 1]);
+                    m4[c + 2] = max_three(m4[c + 2], sv[c][i + 2], sv[c][i + 3]);
+                }
             const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            const bool raise = (m - m_ref) * sl > RAISE;
             bool rest = OVER || j == 0;                   // the last product is known to be complete
-            if (__any_sync(0xffffffffu, raise)) {
+            if (any_of_pair(pair, (m - m_ref) * sl > RAISE)) {
                 if (!rest) {
-                    if (ok) ok = mbar_wait(&o_done[x], (j - 1) & 1, status);
+                    if (ok) ok = wait(&o_done[x], (j - 1) & 1, status);
                     after_sync();
                     rest = true;
                 }
-                const float f = raise ? exp2_fast((m_ref - m) * sl) : 1.0f;
+                *mine = m;
+                sync_pair(pair);
+                const float top = fmaxf(m, *other);       // of the row
+                const bool raise = (top - m_ref) * sl > RAISE;
+                const float f = raise ? exp2_fast((m_ref - top) * sl) : 1.0f;
                 if (j > 0) {
 #pragma unroll 1
                     for (int c = 0; c < D / 32; ++c) {
-                        unsigned ov[32];
-                        tmem_load_32cols(o_addr + 32 * c, ov);
+                        unsigned ov[16];
+                        tmem_load_16cols(o_addr + 16 * c, ov);
                         tmem_wait_loads();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
+                        for (int i = 0; i < 16; ++i)
                             ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
-                        tmem_store_32cols(o_addr + 32 * c, ov);
+                        tmem_store_16cols(o_addr + 16 * c, ov);
                     }
                     tmem_wait_stores();
+                    before_sync();
                 }
                 l_run *= f;
-                if (raise) m_ref = m;
+                if (raise) m_ref = top;
+                sync_pair(pair);                          // both halves are rescaled before a product
             }
             const float off = m_ref == -INFINITY ? 0.0f : -m_ref * sl;
-            float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            unsigned pw[2][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float a = exp2_fast(fmaf(__uint_as_float(sv[c][i]), sl, off));
-                    const float b = exp2_fast(fmaf(__uint_as_float(sv[c][i + 1]), sl, off));
-                    l4[i & 2] += a;
-                    l4[(i & 2) + 1] += b;
-                    pw[c >> 1][(c & 1) * 16 + i / 2] = pack2(a, b);
-                }
-            l_run += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+            const Two sl2 = two(sl, sl), off2 = two(off, off);
             if (!rest) {                                  // the weights' columns are free
-                if (ok) ok = mbar_wait(&o_done[x], (j - 1) & 1, status);
+                if (ok) ok = wait(&o_done[x], (j - 1) & 1, status);
                 after_sync();
             }
-            tmem_store_32cols(p_addr, pw[0]);
-            tmem_store_32cols(p_addr + 32, pw[1]);
-            // values that no row sees may be anything, and 0 * NaN is NaN in the product: thread i has
-            // row i (both pipelines write the same zeros)
-            if (kt + rowi >= it.end || (gone >> (rowi / box) & 1)) {
-                const int unit = 2 * t + 1, b = unit % BUFFERS;
-                if (ok) ok = mbar_wait(&full[b], (unit / BUFFERS) & 1, status);
+            Two sum2[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
 #pragma unroll
-                for (int sub = 0; sub < KS; ++sub) {
-                    uint4* v = reinterpret_cast<uint4*>(ring + b * BUFFER + sub * SUB + rowi * 128);
+            for (int c = 0; c < 2; ++c) {
+                unsigned pw[16];
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) v[c] = make_uint4(0u, 0u, 0u, 0u);
+                for (int i = 0; i < 16; ++i) {
+                    float a, b;
+                    untwo(fma_two(two(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1])),
+                                  sl2, off2), a, b);
+                    a = exp2_fast(a);
+                    b = exp2_fast(b);
+                    sum2[i & 1] = add_two(sum2[i & 1], two(a, b));
+                    pw[i] = pack2(a, b);
                 }
-                asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                tmem_store_16cols(p_addr + 32 * c, pw);
+                if (c == 0) {
+                    // Values that no row sees may be anything, and 0 * NaN is NaN in the product: the
+                    // first thread of row i has the values of key i (both pipelines write the same zeros).
+                    if (EDGE && half == 0 && (kt + rowi >= it.end || (gone >> (rowi / box) & 1))) {
+                        const int unit = 2 * t + 1, b = unit % BUFFERS;
+                        if (ok) ok = wait(&full[b], (unit / BUFFERS) & 1, status);
+#pragma unroll
+                        for (int sub = 0; sub < KS; ++sub) {
+                            uint4* v = reinterpret_cast<uint4*>(ring + b * BUFFER + sub * SUB + rowi * 128);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    }
+                    tmem_wait_stores();
+                    before_sync();
+                    mbar_arrive(&p_half[x]);
+                }
+            }
+            {
+                float a, b;
+                untwo(add_two(sum2[0], sum2[1]), a, b);
+                l_run += a + b;
             }
             tmem_wait_stores();
             before_sync();
             mbar_arrive(&p_ready[x]);
+        };
+        for (int j = 0; j < n_of[x]; ++j) {
+            if (missing || it.begin + (tile_of(x, j) + 1) * KT > it.end) tile(j, Truth<true>());
+            else tile(j, Truth<false>());
         }
-        const int base = it.base + x * LANES + rowi;
-        const size_t at = (size_t)base * kv_heads + hk;
         if (n_of[x] > 0) {
-            if (ok) ok = mbar_wait(&o_done[x], (n_of[x] - 1) & 1, status);
+            if (ok) ok = wait(&o_done[x], (n_of[x] - 1) & 1, status);
             after_sync();
+        }
+        // The rows' results go out by way of the ring (which nobody reads any more when both pipelines
+        // are through): half a row is one bulk copy of its own.
+        *mine = l_run;
+        asm volatile("bar.sync 9, %0;\n" ::"n"(SOFTMAX_WARPS * 32) : "memory");
+        const size_t at = (size_t)(it.base + x * LANES + rowi) * kv_heads + hk;
+        if (n_of[x] > 0) {
+            unsigned char* res = ring + (x * LANES + rowi) * ROW_BYTES + half * D * 2;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-                unsigned ov[32];
-                tmem_load_32cols(o_addr + 32 * c, ov);
+                unsigned ov[16];
+                tmem_load_16cols(o_addr + 16 * c, ov);
                 tmem_wait_loads();
-                if (!ok || !live) continue;
-                uint4* dst = reinterpret_cast<uint4*>(partial_acc + at * D + 32 * c);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    dst[i] = make_uint4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<uint4*>(res + 64 * c + 16 * i) =
+                        make_uint4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
             }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            if (ok && live)
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n"
+                             ::"l"(partial_acc + at * D + D / 2 * half), "r"(smem_u32(res)), "n"(D * 2)
+                             : "memory");
+            asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
         }
         // (nothing where a wait ran out: such a row's results are those of the other ranges)
-        if (live)
-            partial_ml[at] = n_of[x] > 0 && ok ? make_float2(m_ref * sl, l_run)
+        if (live && half == 0)
+            partial_ml[at] = n_of[x] > 0 && ok ? make_float2(m_ref * sl, l_run + *other)
                                                : make_float2(-INFINITY, 0.0f);
+        asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
     }
     before_sync();
     __syncthreads();

@@ -49,6 +49,7 @@ MODULES: dict[str, tuple[str, tuple[str, ...]]] = {
     "sublayer": ("sublayer.cu", ()),
     "beam": ("beam.cu", ()),
     "shared_prefix": ("shared_prefix.cu", ()),
+    "shared_prefix_f32": ("shared_prefix_f32.cu", ()),
     "shared_prefix_mma": ("shared_prefix_mma.cu", ()),  # built per head size: HEAD_DIM=<d>
     "shared_prefix_tcgen05": ("shared_prefix_tcgen05.cu", ()),      # built per head size: 64 and 128
 }

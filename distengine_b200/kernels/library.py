@@ -161,10 +161,14 @@ SIGNATURES: dict[str, dict[str, list]] = {
     },
     "shared_prefix": {
         "de_shared_rows": [I, P, I, P, P, P, I, I, P, P, P, I, I, I, I, P, P, I, I, I, I, F, P, P],
-        "de_shared_merge": [I, P, I, P, P, P, P, I, I, I, I, P],
+        "de_shared_merge_most": [], "de_shared_merge": [I, P, I, P, P, P, P, I, I, I, I, P],
+    },
+    "shared_prefix_f32": {
+        "de_shared_f32_unit": [], "de_shared_f32_held": [I, I],
+        "de_shared_f32": [P, I, P, P, P, I, I, P, P, P, I, I, I, P, P, I, I, I, I, F, P, P],
     },
     "shared_prefix_mma": {
-        "de_shared_mma_rows": [], "de_shared_mma_blocks_per_sm": [],
+        "de_shared_mma_rows": [], "de_shared_mma_unit": [], "de_shared_mma_held": [],
         "de_shared_mma": [P, I, P, P, P, I, I, P, P, P, I, I, I, P, P, I, I, I, I, F, P, P],
     },
     "shared_prefix_tcgen05": {

@@ -22,7 +22,7 @@ from . import library
 from .attention import check_head_dim, uses_tensor_cores
 from .ops import _check, _need, _on_device, _status_word, _stream, _tag
 
-MAX_SPLITS = 256
+MAX_SPLITS = 256         # ranges that a prefix or a request's own keys are cut into
 
 
 @dataclass
@@ -48,26 +48,29 @@ class SharedPlan:
 @dataclass(frozen=True)
 class Tile:
     """A tile of a kernel: the kernel's name among the plan's items, query rows, keys that a range is a
-    multiple of (one number for all tiles of a kernel), blocks that the device holds at once; ``places``:
-    partial results that a range leaves."""
+    multiple of (one number for all tiles of a kernel), blocks (or warps, where those have an item
+    each) that the device holds at once; ``places``: partial results that a range leaves; ``least``: keys
+    of the shortest range that is worth a block."""
     name: str
     rows: int
     unit: int
     blocks: int
     places: int = 1
+    least: int = 1
 
 
-def choose_range(lengths: np.ndarray, copies: np.ndarray, unit: int, blocks: int) -> int:
-    """How long the ranges are that ``lengths`` are cut into, a multiple of ``unit``: range r of length i
-    is the work of ``copies[i]`` blocks.  Of all numbers of rounds of ``blocks`` blocks the one that is
-    done first, a block costing its keys and as much as ``OVERHEAD`` keys besides."""
-    longest = int(lengths.max(initial=0))
+def choose_range(lengths: np.ndarray, copies: np.ndarray, tile: Tile) -> int:
+    """How long the ranges are that ``lengths`` are cut into, a multiple of the tile's unit: each range of
+    length i is the work of ``copies[i]`` blocks.  Of all numbers of rounds of as many blocks as the device
+    holds the one that is done first, a block costing its keys and as much as ``OVERHEAD`` keys besides."""
+    longest, unit, blocks = int(lengths.max(initial=0)), tile.unit, tile.blocks
     whole = -(-longest // unit) * unit
     best = None
+    fewest = max(1, -(-longest // (MAX_SPLITS * unit)), -(-min(tile.least, whole) // unit))
     count = lambda each: int((-(-lengths // each) * copies).sum())
     least = -(-count(max(whole, unit)) // blocks)
     for rounds in range(max(least, 1), max(least, 1) + 4):
-        low, high = 1, max(whole // unit, 1)              # the shortest that needs no more rounds
+        low, high = fewest, max(whole // unit, fewest)    # the shortest that needs no more rounds
         while low < high:
             mid = (low + high) // 2
             if count(mid * unit) <= rounds * blocks:
@@ -83,12 +86,13 @@ def choose_range(lengths: np.ndarray, copies: np.ndarray, unit: int, blocks: int
 OVERHEAD = 256
 
 
+
 def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, prefix_tile,
                 own_tile, tail: int = 0) -> SharedPlan:
     """``seq_qlen``: tokens that each request brings; ``group_sizes``: how many requests, in their
     order, share a prefix; ``prefix_lens``: its keys (0: they share nothing); ``group``: query heads a
-    kv head.  ``prefix_tile``: rows -> ``Tile`` for a group of that many rows; ``own_tile`` the same
-    for one request's own keys.  ``tail``: about how many keys of its own a request has at most (how
+    kv head.  ``prefix_tile``: (rows, keys) -> ``Tile`` for a group of that many rows and its prefix;
+    ``own_tile`` the same for one request's own keys.  ``tail``: about how many keys of its own a request has at most (how
     many ranges they are cut into goes by it, not which keys are seen)."""
     qlen = np.asarray(seq_qlen, dtype=np.int64).reshape(-1)
     sizes = np.asarray(group_sizes, dtype=np.int64).reshape(-1)
@@ -119,12 +123,12 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
     # shared keys
     by_name: dict[str, list] = {}
     for g in np.nonzero((prefix > 0) & (rows > 0))[0]:
-        t = prefix_tile(int(rows[g]))
+        t = prefix_tile(int(rows[g]), int(prefix[g]))
         by_name.setdefault(t.name, []).append((int(g), t))
     for members in by_name.values():
         lengths = prefix[[g for g, _ in members]]
         copies = np.asarray([-(-int(rows[g]) // t.rows) * kv_heads for g, t in members])
-        each = choose_range(lengths, copies, members[0][1].unit, members[0][1].blocks)
+        each = choose_range(lengths, copies, members[0][1])
         for g, t in members:
             p, n = int(prefix[g]), int(rows[g])
             chunks, count = -(-p // each), -(-n // t.rows)
@@ -149,12 +153,12 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
     own = np.maximum(int(tail), qlen) + np.where(start > 0, 0, np.repeat(shared, sizes))
     by_tile: dict[Tile, list] = {}
     for s in np.nonzero(qlen > 0)[0]:
-        by_tile.setdefault(own_tile(int(qlen[s]) * group), []).append(int(s))
+        by_tile.setdefault(own_tile(int(qlen[s]) * group, int(own[s])), []).append(int(s))
     for t, members in by_tile.items():
         s = np.asarray(members)
         n = qlen[s] * group
         count = -(-n // t.rows)
-        each = choose_range(own[s], count * kv_heads, t.unit, t.blocks)
+        each = choose_range(own[s], count * kv_heads, t)
         splits = np.clip(-(-own[s] // each), 1, MAX_SPLITS)
         pieces = count * splits
         owner = np.repeat(np.arange(len(s)), pieces)
@@ -171,7 +175,9 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
         seqs[s, 5], seqs[s, 6], seqs[s, 7] = begin, splits, t.rows
         base += int((pieces * t.rows).sum())
     _need(base < 1 << 31, "shared prefix: too many partial results")
-    return SharedPlan({name: np.concatenate(parts) for name, parts in items.items()}, shapes, seqs,
+    # (the tcgen05 kernel's blocks first: the others' fill the SMs that those leave)
+    names = sorted(items, key=lambda name: (name != "tcgen05", name))
+    return SharedPlan({name: np.concatenate(items[name]) for name in names}, shapes, seqs,
                       np.repeat(np.arange(len(qlen)), qlen), base, total)
 
 
@@ -204,35 +210,48 @@ class SharedPrefixAttention:
             self._sms = int(torch.cuda.get_device_properties(device).multi_processor_count)
         return self._sms
 
-    def tiles(self) -> "tuple":
-        """(rows of a group -> ``Tile``, rows of a request -> ``Tile``)."""
+    def tiles(self, page: "int | None" = None) -> "tuple":
+        """(rows of a group, keys that they share) -> ``Tile``, and the same for one request."""
         sms = self._sm_count()
+        if self.dtype == torch.float32 and self.head_dim % 4 == 0:
+            lib = library.load("shared_prefix_f32")
+            tiles = {rows: Tile(f"f32x{rows}", rows, lib.de_shared_f32_unit(),
+                                lib.de_shared_f32_held(rows, self.head_dim) * sms)
+                     for rows in (8, 16, 32)}
+            tile = lambda rows, keys: tiles[8 if rows <= 8 else 16 if rows <= 16 else 32]
+            return tile, tile
         if not self.tensor_cores:
             plain = Tile("rows", 8, 32, 4 * sms)
-            return (lambda rows: plain), (lambda rows: plain)
+            return (lambda rows, keys: plain), (lambda rows, keys: plain)
         lib = library.load(*self.mma_module)
-        most, blocks = lib.de_shared_mma_rows(), lib.de_shared_mma_blocks_per_sm() * sms
+        unit = lib.de_shared_mma_unit()
+        few = Tile("warp", lib.de_shared_mma_rows(), unit, lib.de_shared_mma_held() * sms, least=4 * unit)
+        wide = self.tcgen05_module is not None and (
+            page is None or library.load(*self.tcgen05_module).de_shared_tcgen05_page_ok(page))
 
-        def few(rows: int) -> Tile:
-            return Tile("mma", min(most, -(-rows // 16) * 16), 64, blocks)
+        def shared(rows: int, keys: int) -> Tile:
+            # (us, tcgen05 and two tiles of the other: 24 rows, 6 groups behind 1,216 keys of 32 kv heads
+            # 55.5 and 39.7; 20 rows behind 2,040 of 8 17.9 and 18.7; 37 rows behind 6,373 of 32 40.6 and,
+            # three tiles, 44.2; 48 rows behind 1,214 of 4, head size 64, 16.0 and 12.5)
+            if rows > 32 and wide:
+                return (Tile("tcgen05", 128, 128, sms, 2) if rows <= 128 else
+                        Tile("tcgen05", 256, 128, sms))
+            return few
 
-        def many(rows: int) -> Tile:
-            if rows <= most or self.tcgen05_module is None:
-                return few(rows)
-            return (Tile("tcgen05", 128, 128, sms, 2) if rows <= 128 else
-                    Tile("tcgen05", 256, 128, sms))
+        return shared, lambda rows, keys: few
 
-        return many, few
-
-    def host_plan(self, seq_qlen, group_sizes, prefix_lens, tail: int = 0) -> SharedPlan:
-        prefix_tile, own_tile = self.tiles()
+    def host_plan(self, seq_qlen, group_sizes, prefix_lens, tail: int = 0,
+                  page: "int | None" = None) -> SharedPlan:
+        prefix_tile, own_tile = self.tiles(page)
         return plan_shared(seq_qlen, group_sizes, prefix_lens, self.group, self.kv_heads, prefix_tile,
                            own_tile, tail)
 
-    def plan(self, seq_qlen, group_sizes, prefix_lens, tail: int = 0) -> SharedPlan:
-        """The plan of a step (arguments as ``plan_shared``) on the device.  It holds for every step
-        of these requests in which they bring the same numbers of tokens."""
-        return self.host_plan(seq_qlen, group_sizes, prefix_lens, tail).to(
+    def plan(self, seq_qlen, group_sizes, prefix_lens, tail: int = 0,
+             page: "int | None" = None) -> SharedPlan:
+        """The plan of a step (arguments as ``plan_shared``; ``page``: keys of the cache's pages, which
+        not all kernels suit) on the device.  It holds for every step of these requests in which they
+        bring the same numbers of tokens."""
+        return self.host_plan(seq_qlen, group_sizes, prefix_lens, tail, page).to(
             self._device if self._device is not None else "cuda")
 
     # ------------------------------------------------------------------ device side
@@ -291,7 +310,10 @@ class SharedPrefixAttention:
                     and (kernel := library.load(*self.tcgen05_module)).de_shared_tcgen05_page_ok(
                         k_pages.shape[2])):
                 _check(kernel.de_shared_tcgen05(*before, *after), "shared prefix attention (tcgen05)")
-            elif name != "rows" and aligned:
+            elif name.startswith("f32") and pages_fit:
+                _check(library.load("shared_prefix_f32").de_shared_f32(*before, rows, behind, *after),
+                       "shared prefix attention (float32)")
+            elif name in ("warp", "tcgen05") and aligned:
                 _check(library.load(*self.mma_module).de_shared_mma(*before, rows, behind, *after),
                        "shared prefix attention (mma)")
             else:

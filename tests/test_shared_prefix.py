@@ -73,8 +73,8 @@ def _seen(plan, tiles, group, kv_heads, qlen, sizes, prefix, own):
 def test_every_key_once(tiles, step, group, kv_heads, tail):
     qlen, sizes, prefix, own = STEPS[step]
     wide, narrow = TILES[tiles]
-    plan = plan_shared(qlen, sizes, prefix, group, kv_heads, lambda rows: wide, lambda rows: narrow,
-                       tail)
+    plan = plan_shared(qlen, sizes, prefix, group, kv_heads, lambda rows, keys: wide,
+                       lambda rows, keys: narrow, tail)
     assert plan.tokens == sum(qlen) and plan.token_seq.tolist() == sum(
         ([s] * n for s, n in enumerate(qlen)), [])
     by_row, pos0, tok0 = _seen(plan, {wide, narrow}, group, kv_heads, qlen, sizes, prefix, own)
@@ -100,7 +100,8 @@ def test_every_key_once(tiles, step, group, kv_heads, tail):
 def test_the_shared_prefix_is_read_once():
     """The keys that the items of a group's prefix name are the prefix, once a tile of rows."""
     wide, narrow = TILES["two"]
-    plan = plan_shared([1] * 16, [16], [5000], 8, 8, lambda rows: wide, lambda rows: narrow, 32)
+    plan = plan_shared([1] * 16, [16], [5000], 8, 8, lambda rows, keys: wide,
+                       lambda rows, keys: narrow, 32)
     shared = plan.items["wide"]
     assert int((shared[:, 5] - shared[:, 4]).sum()) == 5000      # 128 rows: one tile
     assert (plan.items["narrow"][:, 4] == 5000).all()
@@ -108,7 +109,7 @@ def test_the_shared_prefix_is_read_once():
 
 def test_refused_plans():
     tile = TILES["one"][0]
-    make = lambda *a, **k: plan_shared(*a, 4, 2, lambda r: tile, lambda r: tile, **k)
+    make = lambda *a, **k: plan_shared(*a, 4, 2, lambda r, k: tile, lambda r, k: tile, **k)
     for args in (([1, 1], [1], [5]), ([1, 1], [2, 0], [5, 5]), ([1, -1], [2], [5]),
                  ([1, 1], [2], [5, 6]), ([1, 1], [2], [-5]), ([1, 1], [3, -1], [5, 5])):
         with pytest.raises(ValueError, match="shared prefix"):
@@ -135,8 +136,8 @@ def _call(**changed):
     heads, kv_heads, d = 4, 2, 16
     layer = SharedPrefixAttention(torch.float32, heads, kv_heads, d, 0.25, "cpu")
     tile = TILES["one"][0]
-    plan = plan_shared([1, 1], [2], [16], heads // kv_heads, kv_heads, lambda r: tile,
-                       lambda r: tile).to("cpu")
+    plan = plan_shared([1, 1], [2], [16], heads // kv_heads, kv_heads, lambda r, k: tile,
+                       lambda r, k: tile).to("cpu")
     args = dict(q=torch.zeros(2, heads * d), out=torch.zeros(2, heads * d),
                 k_pages=torch.zeros(4, kv_heads, 16, d), v_pages=torch.zeros(4, kv_heads, 16, d),
                 block_table=torch.zeros(2, 2, dtype=torch.int32),
@@ -164,6 +165,7 @@ def test_refused_calls(name, value):
 def test_a_call_off_the_current_device_is_refused():
     with pytest.raises(ValueError, match="current CUDA device"):
         _call()
-    plan = plan_shared([1, 1], [2], [16], 2, 2, lambda r: TILES["one"][0], lambda r: TILES["one"][0])
+    plan = plan_shared([1, 1], [2], [16], 2, 2, lambda r, k: TILES["one"][0],
+                       lambda r, k: TILES["one"][0])
     with pytest.raises(ValueError, match="not on the device"):
         _call(plan=plan)
