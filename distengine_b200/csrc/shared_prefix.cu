@@ -148,14 +148,12 @@ template <typename T, int LANES, bool VEC>
 __global__ void __launch_bounds__(128)
 shared_merge_kernel(T* __restrict__ out, int out_stride, const int* __restrict__ token_seq,
                     const Joined* __restrict__ seqs, const float* __restrict__ partial_acc,
-                    const float2* __restrict__ partial_ml, int tokens, int heads, int kv_heads,
-                    int d) {
+                    const float2* __restrict__ partial_ml, int heads, int kv_heads, int d) {
     constexpr int AT_ONCE = 32 / LANES, N = VEC ? 4 : 8, DEEP = VEC ? 4 : 1;
     __shared__ float weight_s[4][MERGE_MOST];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * 4 + warp;
-    const bool there = unit < (long long)tokens * heads;
-    const int token = there ? (int)(unit / heads) : 0, h = (int)(unit % heads);
+    const int token = blockIdx.x, h = blockIdx.y * 4 + warp;
+    const bool there = h < heads;
     const int g = heads / kv_heads, hk = h / g;
     const Joined s = seqs[token_seq[token]];
     // the results of a row lie a tile's rows apart: the prefix's, then its own keys'
@@ -244,9 +242,8 @@ int merge_of(void* out, int out_stride, const int* token_seq, const int* seqs, c
     const auto kernel = d == 128  ? shared_merge_kernel<T, 32, true>
                         : d == 64 ? shared_merge_kernel<T, 16, true>
                                   : shared_merge_kernel<T, 32, false>;
-    return de_launch(kernel, dim3((unsigned)(((long long)tokens * heads + 3) / 4)), dim3(128), 0, stream,
-                     (T*)out, out_stride, token_seq, (const Joined*)seqs, partial_acc,
-                     (const float2*)partial_ml, tokens, heads, kv_heads, d);
+    return de_launch(kernel, dim3((unsigned)tokens, (heads + 3) / 4), dim3(128), 0, stream, (T*)out, out_stride, token_seq, (const Joined*)seqs, partial_acc,
+                     (const float2*)partial_ml, heads, kv_heads, d);
 }
 
 template <typename T>

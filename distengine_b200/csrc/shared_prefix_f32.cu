@@ -68,21 +68,33 @@ shared_f32_kernel(const float* __restrict__ q, int q_stride, const float* __rest
         }
         row_s[t & 1][tid] = at;
     };
+    // rows of d features go by in pieces of four, a thread every 128th of them
+    const int first_j = tid / pieces, first_f = tid - first_j * pieces;
+    const int step_j = THREADS / pieces, step_f = THREADS - step_j * pieces;
+    auto over_pieces = [&](int rows, auto each) {
+        for (int j = first_j, f = first_f; j < rows;) {
+            each(j, 4 * f);
+            j += step_j;
+            f += step_f;
+            if (f >= pieces) { f -= pieces; ++j; }
+        }
+    };
     auto copy = [&](int t, const float* pages, float* to, int stride) {
         if (t < tiles)
-            for (int c = tid; c < KT * pieces; c += THREADS) {
-                const int j = c / pieces, f = (c - j * pieces) * 4;
+            over_pieces(KT, [&](int j, int f) {
                 const long long at = row_s[t & 1][j];
                 copy16(to + j * stride + f, pages + (at < 0 ? 0 : at + f), at >= 0);
-            }
+            });
         copies_end();
     };
     look_up(0);
-    for (int i = tid; i < ROWS * d; i += THREADS) {
-        const int row = i / d, r = it.row0 + row;
-        q_s[i] = row < it.count ? q[(size_t)(it.tok0 + r / g) * q_stride + (hk * g + r % g) * d + i % d]
-                                : 0.0f;
-    }
+    over_pieces(ROWS, [&](int row, int f) {
+        const int r = it.row0 + row;
+        const float* src = q + (size_t)(it.tok0 + r / g) * q_stride + (hk * g + r % g) * d + f;
+        const bool live = row < it.count;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q_s[row * d + f + e] = live ? src[e] : 0.0f;
+    });
     __syncthreads();
     copy(0, k_pages, k_s, ld);
     copy(0, v_pages, v_s, d);
