@@ -12,10 +12,11 @@ from .registry import register_architecture  # noqa: E402
 def __getattr__(name):
     # the engine pulls in the kernels; load it on first use so that configuration, weights and
     # cache bookkeeping import without a GPU
-    if name in ("Engine", "generate_greedy"):
+    if name in ("Engine", "generate_beam", "generate_greedy"):
         from .engine import engine as _engine
         return getattr(_engine, name)
     raise AttributeError(name)
 
 
-__all__ = ["Engine", "EngineConfig", "LlamaConfig", "generate_greedy", "register_architecture"]
+__all__ = ["Engine", "EngineConfig", "LlamaConfig", "generate_beam", "generate_greedy",
+           "register_architecture"]

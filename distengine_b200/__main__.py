@@ -7,7 +7,8 @@ reference downloads its model and tokenizer; here ``--model`` names a folder (or
 names a config.json, for which a random-weights model folder is written into a temporary folder
 from ``--weights-seed``), ``--prompt-ids`` gives token ids directly, and ``--prompt`` needs a
 ``tokenizer.json`` in the model folder.
-``--decode-batch-size`` is the reference's benchmark flag (src/utils/benchmark.py:593).
+``--decode-batch-size`` is the reference's benchmark flag (src/utils/benchmark.py:593).  ``--beams``
+runs a beam search instead, which the reference does not have.
 ``random-model`` writes a model folder from a configuration and a seed.
 ``bench`` runs a set of requests with arrival times through the engine and reports what the
 reference's benchmark reports of its requests (src/utils/benchmark.py:585-609: ``--repeats``,
@@ -41,6 +42,8 @@ def _with_model_folder(args: argparse.Namespace, run) -> int:
     with random weights for ``--random CONFIG``."""
     if args.max_new_tokens <= 0:
         raise SystemExit("--max-new-tokens must be positive")
+    if getattr(args, "beams", 1) < 1 or getattr(args, "beams", 1) > 1 and args.temperature:
+        raise SystemExit("--beams must be positive, and above 1 without --temperature")
     if (args.model is None) == (args.random is None):
         raise SystemExit("give either --model DIR or --random CONFIG.json")
     scratch = None
@@ -141,9 +144,16 @@ def _generate_from_folder(args: argparse.Namespace) -> int:
     if eos is None:
         eos = engine.model.config.eos_token_id if getattr(engine.model.config, "eos_token_id",
                                                           None) is not None else -1
-    outputs = engine.generate(prompts, args.max_new_tokens, eos, args.temperature, args.seed)
-    for generated in outputs:
+    if args.beams > 1:
+        found = engine.beam_search(prompts, args.max_new_tokens, args.beams, eos, args.length_penalty)
+        outputs = [hypotheses[0].token_ids for hypotheses in found]
+    else:
+        found = None
+        outputs = engine.generate(prompts, args.max_new_tokens, eos, args.temperature, args.seed)
+    for i, generated in enumerate(outputs):
         print("Generated token IDs:", generated)
+        if found is not None:
+            print(f"Score: {found[i][0].score:.4f}")
         if tokenizer is not None:
             print(tokenizer.decode(generated, skip_special_tokens=True))
     return 0
@@ -181,6 +191,10 @@ def main(argv: "list[str] | None" = None) -> int:
     gen.add_argument("--max-new-tokens", type=int, default=32)
     gen.add_argument("--temperature", type=float, default=0.0, help="0: greedy")
     gen.add_argument("--seed", type=int, default=0, help="sampling seed of the first prompt")
+    gen.add_argument("--beams", type=int, default=1,
+                     help="above 1: beam search; the best of this many beams is printed")
+    gen.add_argument("--length-penalty", type=float, default=1.0,
+                     help="of a beam search: a score is the log probability over the length to this power")
     gen.add_argument("--eos-token-id", type=int, default=None,
                      help="default: the configuration's, else none (-1)")
     gen.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])

@@ -15,6 +15,10 @@ group of layers, and slots for per-request state of fixed size.
 * Pages are taken when a step is about to write positions (``reserve``, all requests of the step
   or none) and given back at ``release`` or when a window has passed them (``commit``).  The free
   list is last-in first-out, so pages are used again at once.
+* A request may be *forked*: the copy shares all pages that are filled (a page counts its holders and
+  is free when the last one gave it back) and has a page of its own for the unfilled one and state rows
+  of its own, copied on the device.  ``reorder`` makes requests of one length take over each other's
+  contents at once, as the beams of a search do; only unfilled pages and state rows move.
 * A step may be launched before its caller knows that it counts (the engine keeps the GPU one
   decode step ahead of the host).  Such a step is committed *tentatively*: lengths advance, but no
   page that a window has passed is given back and the state rows of its requests are copied aside
@@ -49,14 +53,15 @@ class OutOfSlots(RuntimeError):
 
 class PagePool:
     """Free list of one group.  ``take`` pops from the end, ``give`` appends: last in, first
-    out."""
+    out.  ``share`` gives a held page another holder; it is free when all have given it back."""
 
     def __init__(self, num_pages: int) -> None:
         if type(num_pages) is not int or num_pages <= 0:
             raise ValueError("num_pages must be a positive integer")
         self.num_pages = num_pages
         self._free = list(range(num_pages))
-        self._held = [False] * num_pages
+        self._held = [0] * num_pages          # holders of each page
+        self.num_shared = 0                   # pages with more than one
 
     @property
     def num_free(self) -> int:
@@ -67,15 +72,31 @@ class PagePool:
             raise OutOfPages(f"{count} pages wanted, {len(self._free)} free")
         pages = [self._free.pop() for _ in range(count)]
         for p in pages:
-            self._held[p] = True
+            self._held[p] = 1
         return pages
 
-    def give(self, pages: list[int]) -> None:
+    def share(self, pages: list[int]) -> None:
+        for p in pages:
+            if not 0 <= p < self.num_pages or not self._held[p]:
+                raise KeyError(f"page {p} is not held: it cannot be shared")
+            self._held[p] += 1
+            self.num_shared += self._held[p] == 2
+
+    def give(self, pages: list[int]) -> "list[int]":
+        """Returns the pages that are free now."""
+        gone = []
         for p in pages:
             if not 0 <= p < self.num_pages or not self._held[p]:
                 raise KeyError(f"page {p} is not held: it cannot be given back")
-            self._held[p] = False
-            self._free.append(p)
+            self._held[p] -= 1
+            self.num_shared -= self._held[p] == 1
+            if not self._held[p]:
+                self._free.append(p)
+                gone.append(p)
+        return gone
+
+    def holders(self, page: int) -> int:
+        return self._held[page]
 
     def free_pages(self) -> list[int]:
         return list(self._free)
@@ -401,9 +422,137 @@ class CacheManager:
         self.slots.give(live.slot)
         del self.live[request_id]
 
+    # ------------------------------------------------------------------ shared contents
+    def fork(self, request_id: str, copies: "list[str]") -> None:
+        """Admit ``copies``, requests that hold what ``request_id`` holds: its filled pages with it, an
+        unfilled page and state rows of their own with the same contents (copied on the current
+        stream).  All of them or, where slots or pages are too few, none."""
+        live = self._get(request_id)
+        if live.confirmed is not None:
+            raise ValueError(f"request '{request_id}' has a tentative step: confirm or rewind it "
+                             f"before it is forked")
+        if len(set(copies)) != len(copies):
+            raise ValueError("the copies of a request need names of their own")
+        for name in copies:
+            if not isinstance(name, str) or not name:
+                raise ValueError("request_id must be a nonempty string")
+            if name in self.live:
+                raise ValueError(f"request '{name}' is already live")
+        if len(copies) > self.slots.num_free:
+            raise OutOfSlots(f"{len(copies)} slots wanted, {self.slots.num_free} are free")
+        full, rest = divmod(live.length, self.page_size)
+        need = len(copies) if rest else 0
+        if any(need > g.pool.num_free for g in self.paged):
+            raise OutOfPages(f"{need} pages wanted, {self.num_free_pages()} are free")
+        for name in copies:
+            slot = self.admit(name)
+            self.live[name].length = live.length
+            for group in self.paged:
+                table = group.tables[request_id][: full + (1 if rest else 0)]
+                group.pool.share([p for p in table[:full] if p >= 0])
+                if rest:
+                    table[full] = group.pool.take(1)[0]
+                group.tables[name] = table
+                group.host_table.numpy()[slot, : len(table)] = table
+                self._mark(group, slot, 0, len(table))
+        for i in range(0, len(copies), 31):               # (the most that one reordering moves, with the first)
+            names = [request_id, *copies[i: i + 31]]
+            self._move([names], [[0] * len(names)])
+
+    def reorder(self, groups: "list[list[str]]", parents: "list[list[int]]") -> None:
+        """Every request of a group takes over the contents of its parent, request
+        ``groups[g][parents[g][i]]`` as it was before the call.  The requests of a group have one length
+        and no tentative step; groups are of one size and no request is in two."""
+        for names, source in zip(groups, parents):
+            lengths = {self._get(name).length for name in names}
+            if len(names) != len(source) or len(names) != len(groups[0]) or len(lengths) > 1:
+                raise ValueError("a group's requests have one length and a parent each, and groups one "
+                                 "size")
+            if any(self._get(name).confirmed is not None for name in names):
+                raise ValueError("a request has a tentative step: confirm or rewind it before it is "
+                                 "reordered")
+            if any(type(i) is not int or not 0 <= i < len(names) for i in source):
+                raise ValueError("a parent is a request of the group")
+        flat = [name for names in groups for name in names]
+        if len(groups) != len(parents) or len(set(flat)) != len(flat):
+            raise ValueError("every request is in one group, every group has its parents")
+        if all(i == p for source in parents for i, p in enumerate(source)):
+            return
+        for names, source in zip(groups, parents):
+            full = self._get(names[0]).length // self.page_size
+            for group in self.paged:
+                before = {name: list(group.tables[name]) for name in names}
+                for i, name in enumerate(names):
+                    if source[i] != i:
+                        group.pool.share([p for p in before[names[source[i]]][:full] if p >= 0])
+                for i, name in enumerate(names):
+                    if source[i] == i:
+                        continue
+                    self._give(group, [p for p in before[name][:full] if p >= 0])
+                    table = before[names[source[i]]][:full] + before[name][full:]
+                    group.tables[name] = table
+                    slot = self._get(name).slot
+                    group.host_table.numpy()[slot, : len(table)] = table
+                    self._mark(group, slot, 0, len(table))
+        self._move(groups, parents)
+
+    def _move(self, groups: "list[list[str]]", parents: "list[list[int]]") -> None:
+        """The device's half of a reordering: unfilled pages and state rows."""
+        def move(tensors, slots):
+            if self.device.type == "cuda":
+                from ..kernels import ops
+                rows = torch.tensor(slots, dtype=torch.int32).to(self.device)
+                for tensor in tensors:
+                    ops.beam_reorder(tensor, rows, parent)
+                return
+            to = [(s, row[p]) for row, source in zip(slots, parents) for s, p in zip(row, source) if s >= 0]
+            for tensor in tensors:                        # (tests of the host side)
+                tensor[:, [a for a, _ in to]] = tensor[:, [b for _, b in to]]
+
+        if self.device.type == "cuda":
+            parent = torch.tensor(parents, dtype=torch.int32).to(self.device)
+        for group in self.paged:
+            slots = []
+            for names in groups:
+                full, rest = divmod(self._get(names[0]).length, self.page_size)
+                slots.append([group.tables[name][full] if rest else -1 for name in names])
+            if any(s >= 0 for row in slots for s in row):
+                move([group.k] if group.spec.values_in_keys else [group.k, group.v], slots)
+        if self.states:
+            move([sgroup.state for sgroup in self.states],
+                 [[self._get(name).slot for name in names] for names in groups])
+
+    def shared_prefixes(self, request_ids: "list[str]") -> "tuple[list[int], list[int]] | None":
+        """Runs of these requests, in their order, that begin with the same pages: how many requests
+        each has, and how many keys they share (0 for a request that shares none); None where no page
+        is shared at all."""
+        group = next((g for g in self.paged if not g.spec.releases), None)
+        if group is None or not group.pool.num_shared:
+            return None
+        sizes: list[int] = []
+        shared: list[int] = []
+        first = None
+        for name in request_ids:
+            live = self._get(name)
+            row = group.host_table.numpy()[live.slot, : live.length // self.page_size]
+            if first is not None:
+                n = min(len(row), len(first))
+                differ = np.nonzero(row[:n] != first[:n])[0]
+                common = int(differ[0]) if len(differ) else n
+                if common:
+                    sizes[-1] += 1
+                    shared[-1] = min(common, shared[-1]) if sizes[-1] > 2 else common
+                    continue
+            first = row
+            sizes.append(1)
+            shared.append(0)
+        if max(sizes, default=0) < 2:
+            return None
+        return sizes, [n * self.page_size for n in shared]
+
     def _give(self, group: _PagedGroup, pages: list[int]) -> None:
-        group.pool.give(pages)
-        if self.poison:
+        pages = group.pool.give(pages)
+        if self.poison and pages:
             index = torch.tensor(pages, dtype=torch.long, device=self.device)
             group.k[:, index] = float("nan")
             group.v[:, index] = float("nan")
@@ -471,14 +620,18 @@ class CacheManager:
 
     # ------------------------------------------------------------------ checks (tests)
     def check_invariants(self) -> None:
-        """No page lost, none held twice, tables and free lists add up."""
+        """No page lost, each held as often as the pool says, tables and free lists add up."""
         for group in self.paged:
-            held: list[int] = []
+            held: dict[int, int] = {}
             for table in group.tables.values():
-                held += [p for p in table if p >= 0]
+                for p in table:
+                    if p >= 0:
+                        held[p] = held.get(p, 0) + 1
             free = group.pool.free_pages()
-            if len(set(held)) != len(held):
-                raise AssertionError("a page is held twice")
+            if any(group.pool.holders(p) != n for p, n in held.items()):
+                raise AssertionError("a page is held twice, or by nobody")
+            if sum(n > 1 for n in held.values()) != group.pool.num_shared:
+                raise AssertionError("the pool miscounts its shared pages")
             if set(held) & set(free):
                 raise AssertionError("a page is both held and free")
             if len(held) + len(free) != group.pool.num_pages or len(set(free)) != len(free):

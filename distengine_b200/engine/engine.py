@@ -20,6 +20,7 @@ from ..cache.manager import CacheManager
 from ..config.engine import EngineConfig
 from ..models.loading import load_model
 from ..sampling.sampler import Sampler, pack_sampling
+from .beam import BeamSearch, Hypothesis
 from .request import Request
 from .scheduler import Scheduler
 from .step import StepEntry, StepRunner
@@ -208,11 +209,46 @@ class Engine:
         return [results[rid] for rid in ids]
 
 
+    def beam_search(self, prompts: list[list[int]], max_new_tokens: int, num_beams: int,
+                    eos_token_id: int = -1,
+                    length_penalty: float = 1.0) -> "list[list[Hypothesis]]":
+        """For every prompt (token ids) the ``num_beams`` best continuations that a beam search finds, best
+        first: ``token_ids`` and ``score``, the log probability over (generated tokens) **
+        ``length_penalty`` (``engine.beam``).  The engine must have no pending request."""
+        if self.has_pending():
+            raise RuntimeError("a beam search needs the engine without pending requests")
+        for prompt in prompts:                            # (the same rules as for any request)
+            Request("beam", prompt, max_new_tokens, eos_token_id)
+            self.scheduler.check(prompt, max_new_tokens)
+        search = BeamSearch(self.runner, self.cache, num_beams, self.config.max_batch_tokens,
+                            length_penalty)
+        return search.run([list(p) for p in prompts], max_new_tokens, eos_token_id,
+                          f"beam-{time.monotonic_ns()}")
+
+
+def generate_beam(model, input_ids, max_new_tokens: int, eos_token_id: int, num_beams: int,
+                  length_penalty: float = 1.0, **engine_options) -> torch.Tensor:
+    """``generate_greedy`` with a beam search: ``input_ids`` [1, T] -> [1, T + generated], the best
+    continuation."""
+    engine, ids, prompt = _one_prompt(model, input_ids, max_new_tokens, engine_options)
+    found = engine.beam_search([prompt], max_new_tokens, num_beams, eos_token_id, length_penalty)[0]
+    if not found:
+        raise RuntimeError("the prompt has no continuation (its logits are not finite)")
+    return torch.tensor([prompt + found[0].token_ids], dtype=ids.dtype, device=ids.device)
+
+
 def generate_greedy(model, input_ids, max_new_tokens: int, eos_token_id: int,
                     **engine_options) -> torch.Tensor:
     """``input_ids`` [1, T] -> [1, T + generated], greedily, like the reference's
     ``generate_greedy`` (src/utils/generation.py:49-91); ``model`` is a model folder, a loaded
     model or an ``Engine``."""
+    engine, ids, prompt = _one_prompt(model, input_ids, max_new_tokens, engine_options)
+    generated = engine.generate([prompt], max_new_tokens, eos_token_id)[0]
+    return torch.tensor([prompt + generated], dtype=ids.dtype, device=ids.device)
+
+
+def _one_prompt(model, input_ids, max_new_tokens: int, engine_options: dict):
+    """(engine, the ids as a tensor, the prompt as a list) of a call with one prompt."""
     ids = torch.as_tensor(input_ids)
     if ids.ndim != 2 or ids.shape[0] != 1:
         raise ValueError("Expected input_ids with shape [1, T]")
@@ -221,6 +257,4 @@ def generate_greedy(model, input_ids, max_new_tokens: int, eos_token_id: int,
     if max_new_tokens <= 0:
         raise ValueError("max_new_tokens must be positive")
     engine = model if isinstance(model, Engine) else Engine(model, **engine_options)
-    prompt = [int(t) for t in ids[0].tolist()]
-    generated = engine.generate([prompt], max_new_tokens, eos_token_id)[0]
-    return torch.tensor([prompt + generated], dtype=ids.dtype, device=ids.device)
+    return engine, ids, [int(t) for t in ids[0].tolist()]

@@ -71,21 +71,25 @@ class Scheduler:
         """Validate and enqueue; nothing is allocated (src/distengine/coordinator.py:146-194)."""
         if request.request_id in self.seen_ids:
             raise ValueError("Request ID has already been submitted")
-        for token_id in request.prompt_token_ids:
+        self.check(request.prompt_token_ids, request.max_new_tokens)
+        self.seen_ids.add(request.request_id)
+        self.waiting.append(request)
+
+    def check(self, prompt_token_ids: list[int], max_new_tokens: int) -> None:
+        """Raises where such a request could never run (src/distengine/coordinator.py:146-186)."""
+        for token_id in prompt_token_ids:
             if type(token_id) is not int:
                 raise ValueError("Token IDs must be integers")
             if not 0 <= token_id < self.vocabulary:
                 raise ValueError("Token ID is outside the model vocabulary")
-        most = request.num_prompt_tokens + request.max_new_tokens - 1     # the last token is never cached
+        most = len(prompt_token_ids) + max_new_tokens - 1                 # the last token is never cached
         if most > self.cache.capacity_tokens:
             raise ValueError(f"Request exceeds KV capacity: it may hold {most} tokens, the pool "
                              f"has room for {self.cache.capacity_tokens}")
-        if request.num_prompt_tokens + request.max_new_tokens > self.max_model_len:
+        if len(prompt_token_ids) + max_new_tokens > self.max_model_len:
             raise ValueError(f"Request exceeds the model's length: prompt "
-                             f"{request.num_prompt_tokens} + max_new_tokens "
-                             f"{request.max_new_tokens} > {self.max_model_len}")
-        self.seen_ids.add(request.request_id)
-        self.waiting.append(request)
+                             f"{len(prompt_token_ids)} + max_new_tokens "
+                             f"{max_new_tokens} > {self.max_model_len}")
 
     def has_pending(self) -> bool:
         return bool(self.waiting or self.running)

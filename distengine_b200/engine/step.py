@@ -135,11 +135,13 @@ class StepRunner:
         token_ids = np.concatenate([np.asarray(e.tokens, dtype=np.int32) for e in entries])
         rows = np.array([qstart[i] + w for i, e in enumerate(entries) for w in e.want],
                         dtype=np.int32)
+        ids = [e.request_id for e in entries]
+        shares = getattr(self.cache, "shared_prefixes", None)
         return SimpleNamespace(
             n_tokens=n, n_seqs=s, token_ids=token_ids, positions=pos0[token_seq] + offsets,
             token_slot=slots[token_seq], token_seq=token_seq, seq_slot=slots, seq_qstart=qstart,
             seq_qlen=lens, seq_pos0=pos0, logit_rows=rows,
-            request_ids=[e.request_id for e in entries])
+            request_ids=ids, shared=shares(ids) if shares is not None else None)
 
     _BASE = ("token_ids", "positions", "token_slot", "token_seq", "seq_slot", "seq_qstart",
              "seq_qlen", "seq_pos0", "logit_rows")
@@ -337,6 +339,7 @@ class StepRunner:
             what = {1: "a token's position had no page in its request's block table",
                     2: "a key that a token reads had no page in its request's block table",
                     3: "a bounded wait inside a tcgen05 kernel ran out",
-                    4: "a tcgen05 kernel found its shared memory misaligned"}.get(
+                    4: "a tcgen05 kernel found its shared memory misaligned",
+                    5: "a beam's row or its parent's could not be used"}.get(
                         code, "unknown code")
             raise KernelStatusError(f"a kernel reported status {code}: {what}")

@@ -34,6 +34,7 @@ MAX_HEAD_DIM = 256
 F32_CHUNK = 128          # keys in a chunk of the float32 path (a fixed order of summation)
 _status_fallback: "torch.Tensor | None" = None
 NARROW_ROWS = 16
+SHARED_SAVES = int(os.environ.get("SHARED_SAVES", 4 << 20))
 
 
 def check_head_dim(head_dim: int) -> None:
@@ -59,12 +60,13 @@ class AttentionLauncher:
     def __init__(self, dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int,
                  scale: float, window: "int | None",
                  device: "torch.device | None" = None, exact_weights: bool = False,
-                 extras: bool = False) -> None:
+                 extras: bool = False, share: bool = False) -> None:
         """``exact_weights``: the softmax weights are not rounded to bfloat16 for their product
         with the values: they enter it as two bfloat16 terms (the mma.sync kernel; steps of single
         tokens then never take the one-launch kernel).  ``extras``: the mma.sync kernel's build that
         takes a soft cap, a sink and a factor of the results (``run``); with ``exact_weights`` and a
-        scale above 0."""
+        scale above 0.  ``share``: steps of single tokens whose requests begin with the same pages
+        (``host.shared``) go through ``run_shared`` where that pays."""
         check_head_dim(head_dim)
         if extras and not (exact_weights and scale > 0 and uses_tensor_cores(dtype, head_dim)):
             raise ValueError("attention: extras go with the tensor cores' exact weights and a "
@@ -106,6 +108,14 @@ class AttentionLauncher:
         self.fused_rows = (dtype == torch.float32 and head_dim % 4 == 0 and self.group <= 8
                            and os.environ.get("DISTENGINE_B200_DECODE_ATTENTION",
                                               "fused") != "split")
+        # keys and values that several requests share are read once (kernels.shared_prefix);
+        # DISTENGINE_B200_SHARED_PREFIX=0 has every request read them for itself
+        self.shared = None
+        if (share and scale > 0 and not window and not exact_weights
+                and os.environ.get("DISTENGINE_B200_SHARED_PREFIX", "1") != "0"):
+            from .shared_prefix import SharedPrefixAttention
+            self.shared = SharedPrefixAttention(dtype, heads, kv_heads, head_dim, scale, device)
+        self._shared_plan: "tuple | None" = None            # (what it was made for, the plan)
         self._decode_blocks_per_sm: "int | None" = None     # asked of the kernel at first use
         self._device = device
         self._sm_count: "int | None" = None                 # asked of the device at first use
@@ -159,6 +169,34 @@ class AttentionLauncher:
         tiles = (host.seq_qlen.astype(np.int64) * self.group + 7) // 8
         blocks = int((tiles * ((spans + F32_CHUNK - 1) // F32_CHUNK)).sum()) * self.kv_heads
         return blocks <= (512 if self.head_dim <= 128 else 200)
+
+    def _prepare_shared(self, prep) -> bool:
+        """Whether a step of single tokens goes through ``run_shared``; its work lists, if so."""
+        host = prep.host
+        shared = getattr(host, "shared", None)
+        if self.shared is None or shared is None:
+            return False
+        sizes, prefix = shared
+        saved = sum((n - 1) * p for n, p in zip(sizes, prefix))
+        if saved * 2 * self.kv_heads * self.head_dim * self.dtype.itemsize < SHARED_SAVES:
+            return False
+        # the requests' own keys, as a power of two: the plan holds until they have outgrown it
+        own = int((host.seq_pos0 + 1 - np.repeat(prefix, sizes)).max())
+        tail = max(64, 1 << (own - 1).bit_length())
+        made_for = (tuple(sizes), tuple(prefix), tail, prep.page_size)
+        if self._shared_plan is None or self._shared_plan[0] != made_for:
+            self._shared_plan = (made_for, self.shared.host_plan(
+                host.seq_qlen, sizes, prefix, tail, prep.page_size))
+        plan = self._shared_plan[1]
+        for name, items in plan.items.items():
+            prep.add(f"{self.key}/shared/{name}", items)
+        prep.add(f"{self.key}/shared/seqs", plan.seqs)
+        prep.add(f"{self.key}/shared/token_seq", plan.token_seq)
+        prep.notes[self.key] = ()
+        prep.notes[self.key + "/decode"] = None
+        prep.notes[self.key + "/shared"] = (tuple(plan.shapes.items()), tuple(plan.items),
+                                            plan.partial_rows, plan.tokens)
+        return True
 
     def _prepare_decode(self, prep, force_split: "tuple[int, int, int] | None") -> None:
         """A step in which every sequence brings one token: the work list of the one-launch
@@ -215,6 +253,9 @@ class AttentionLauncher:
             return
         host = prep.host
         one_each = bool(len(host.seq_qlen)) and bool((host.seq_qlen == 1).all())
+        if one_each and force_shape is None and allow_decode and force_split is None \
+                and force_chunk is None and self._prepare_shared(prep):
+            return
         if self.fused_decode and one_each and force_shape is None and allow_decode:
             self._prepare_decode(prep, force_split)
             return
@@ -323,6 +364,22 @@ class AttentionLauncher:
                          shape.rows, acc, ml, self.heads, self.kv_heads, d, self.scale, self.window,
                          getattr(ctx, "status", None), (float(softcap), sink, float(out_scale)))
 
+
+    def shared_step(self, ctx) -> bool:
+        """Whether ``run_shared`` takes this step."""
+        return ctx.notes.get(self.key + "/shared") is not None
+
+    def run_shared(self, q: torch.Tensor, out: torch.Tensor, k_pages: torch.Tensor,
+                   v_pages: torch.Tensor, block_table: torch.Tensor, ctx) -> None:
+        """A step of single tokens whose requests share prefixes; arguments as ``run``."""
+        from .shared_prefix import SharedPlan
+        shapes, names, partial_rows, tokens = ctx.notes[self.key + "/shared"]
+        at = f"{self.key}/shared/"
+        plan = SharedPlan({name: ctx.arrays[at + name] for name in names}, dict(shapes),
+                          ctx.arrays[at + "seqs"], ctx.arrays[at + "token_seq"], partial_rows, tokens,
+                          q.device)
+        self.shared.run(q, out, k_pages, v_pages, block_table, ctx.seq_slot, ctx.seq_pos0, plan,
+                        ctx.status, ctx.buffer)
 
     def decode_step(self, ctx) -> bool:
         """Whether ``run_decode`` takes this step (it then also rotates and stores k and v)."""

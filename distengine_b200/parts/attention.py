@@ -31,7 +31,8 @@ class PagedAttention(Mixer):
         self.width, self.heads, self.kv_heads, self.head_dim = width, heads, kv_heads, head_dim
         self.scale, self.window = float(scale), window
         self.position = build_position_encoding(position, dtype, device)
-        self.kernels = AttentionLauncher(dtype, heads, kv_heads, head_dim, scale, window, device)
+        self.kernels = AttentionLauncher(dtype, heads, kv_heads, head_dim, scale, window, device,
+                                         share=True)
         self.w_qkv: "torch.Tensor | None" = None
         self.w_o: "torch.Tensor | None" = None
 
@@ -92,7 +93,8 @@ class PagedAttention(Mixer):
             ops.rope_kv_write(qkv, ctx.positions, ctx.token_slot, inv_freq, rotary_dim,
                               self.heads, self.kv_heads, d, cache.k_pages, cache.v_pages,
                               cache.block_table, cache.writes, ctx.status)
-            self.kernels.run(qkv, out, cache.k_pages, cache.v_pages, cache.block_table, ctx)
+            run = self.kernels.run_shared if self.kernels.shared_step(ctx) else self.kernels.run
+            run(qkv, out, cache.k_pages, cache.v_pages, cache.block_table, ctx)
         if ahead is not None:          # the product joins the residual and does the next norm's work
             ops.linear(out, self.w_o, out=ahead.rows, status=ctx.status, after=ahead)
             return None
