@@ -578,7 +578,7 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
 
 // Slices that a row is cut into, and their logits: as many blocks as the SMs hold at once (four each),
 // of no fewer than 2,048 logits.  (512 rows of 128,256 in one slice each, 512 blocks; in four, whose
-// ends of a few microseconds are then paid four times, 73 us instead of SELECT_LARGE.)
+// ends of a few microseconds are then paid four times, 73 us instead of 61.)
 struct Slicing {
     int slices, elements;
 };
@@ -601,10 +601,11 @@ size_t aligned(size_t bytes) { return (bytes + 15) & ~(size_t)15; }
 // group in one layer: it reads the pieces of every row that a moved beam takes, and only then writes,
 // so the rows can change places without a buffer.
 // ------------------------------------------------------------------------------------------
-#ifndef REORDER_BLOCKS
-#define REORDER_BLOCKS 16
-#endif
 constexpr int MOVE_THREADS = 256;
+// Blocks of a launch for every SM.  (us for 2, 4, 8 and 16: four beams of sixteen groups, pages of 32 x 16 x 128
+// bfloat16 in 32 layers, 69, 65, 60 and 58; eight beams of eight groups, states of 16 x 128 x 128 floats in six
+// layers, 102, 96, 88 and 85, where a plain copy of the bytes takes 80.)
+constexpr int MOVE_BLOCKS = 16;
 
 // pieces of a row that a thread has under way at once: as many as 64 registers hold for all beams
 template <typename U, int BEAMS> __host__ __device__ constexpr int pieces_at_once() {
@@ -682,7 +683,7 @@ int reorder_with(unsigned char* x, int layers, int pool, long long row_bytes, co
     const long long chunks = (row_bytes + per_chunk - 1) / per_chunk, units = chunks * layers;
     if (units > 0x7fffffffll || groups > 65535) return -4;
     // a block looks the group's moves up once and goes through several chunks
-    long long blocks = (REORDER_BLOCKS * 148 + groups - 1) / groups;
+    long long blocks = (MOVE_BLOCKS * 148 + groups - 1) / groups;
     if (blocks > units) blocks = units;
     return de_launch(beam_reorder_kernel<U, BEAMS>, dim3((unsigned)blocks, groups), dim3(MOVE_THREADS),
                      0, stream, x, row_bytes, pool, slots, parent, groups, beams, (int)chunks,

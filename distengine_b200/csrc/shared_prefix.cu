@@ -27,6 +27,7 @@ constexpr int ROWS = 8;               // query rows of a block
 constexpr int KT = 32;                // keys of a tile
 constexpr int THREADS = 128;
 constexpr int MERGE_MOST = 1024;       // partial results of a row
+constexpr int MERGE_FEW = 8;           // of them a warp reads alone
 
 // A block takes eight rows of an item (blockIdx.y: which), a warp two.  Scores: a lane a key;
 // results: a lane every 32nd feature.
@@ -141,20 +142,24 @@ shared_rows_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ 
     if (behind) pdl_wait();
 }
 
-// A warp a (token, query head).  The lanes take the partial results' maxima and sums in turn, which
-// gives each its weight; then the weighted results are summed, LANES lanes a result (a lane four
+// WARPS warps a (token, query head).  The threads take the partial results' maxima and sums in turn,
+// which gives each its weight; then the weighted results are summed, LANES lanes a result (a lane four
 // features at a time where VEC) and several results at once.
-template <typename T, int LANES, bool VEC>
+template <typename T, int WARPS, int LANES, bool VEC>
 __global__ void __launch_bounds__(128)
 shared_merge_kernel(T* __restrict__ out, int out_stride, const int* __restrict__ token_seq,
                     const Joined* __restrict__ seqs, const float* __restrict__ partial_acc,
                     const float2* __restrict__ partial_ml, int heads, int kv_heads, int d) {
-    constexpr int AT_ONCE = 32 / LANES, N = VEC ? 4 : 8, DEEP = VEC ? 4 : 1;
-    __shared__ float weight_s[4][MERGE_MOST];
+    constexpr int UNITS = 4 / WARPS, GROUP = 32 * WARPS, AT_ONCE = GROUP / LANES;
+    constexpr int N = VEC ? 4 : 8, DEEP = VEC ? 4 : 1;
+    __shared__ float weight_s[UNITS][WARPS == 1 ? MERGE_FEW : MERGE_MOST];
+    __shared__ float top_s[4], total_s[4];
+    __shared__ float sum_s[WARPS == 1 ? 1 : 4][WARPS == 1 ? 1 : (VEC ? 4 * LANES : 256)];
+    const int unit = threadIdx.x / GROUP, tid = threadIdx.x % GROUP;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int token = blockIdx.x, h = blockIdx.y * 4 + warp;
-    const bool there = h < heads;
-    const int g = heads / kv_heads, hk = h / g;
+    const int token = blockIdx.x, h = blockIdx.y * UNITS + unit;
+    const bool there = h < heads;                         // (with one warp a unit; else all are)
+    const int g = heads / kv_heads, hk = (there ? h : 0) / g;
     const Joined s = seqs[token_seq[token]];
     // the results of a row lie a tile's rows apart: the prefix's, then its own keys'
     const int row_p = (token - s.group_tok0) * g + h % g, row_o = (token - s.tok0) * g + h % g;
@@ -174,35 +179,48 @@ shared_merge_kernel(T* __restrict__ out, int out_stride, const int* __restrict__
     pdl_wait();
     pdl_trigger();
     if (!there) return;
-    float top = -INFINITY;
-    for (int c = lane; c < parts; c += 32) top = fmaxf(top, partial_ml[place(c)].x);
+    // (what a thread reads first it keeps: there are seldom more results than threads)
+    float2 first = make_float2(-INFINITY, 0.0f);
+    if (tid < parts) first = partial_ml[place(tid)];
+    float top = first.x;
+    for (int c = tid + GROUP; c < parts; c += GROUP) top = fmaxf(top, partial_ml[place(c)].x);
     top = warp_max(top);
+    if (WARPS > 1) {
+        if (lane == 0) top_s[warp] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(top_s[0], top_s[1]), fmaxf(top_s[2], top_s[3]));
+    }
     if (top == -INFINITY) top = 0.0f;
     float total = 0.0f;
-    for (int c = lane; c < parts; c += 32) {
-        const float2 ml = partial_ml[place(c)];
+    for (int c = tid; c < parts; c += GROUP) {
+        const float2 ml = c == tid ? first : partial_ml[place(c)];
         // (a range without a key has left no result; one of NaN scores only has a sum that is NaN)
         const bool empty = ml.x == -INFINITY && ml.y == 0.0f;
         const float w = empty ? 0.0f : exp2f(ml.x - top);
         total += empty ? 0.0f : w * ml.y;
-        weight_s[warp][c] = empty ? -1.0f : w;
+        weight_s[unit][c] = empty ? -1.0f : w;
     }
     total = warp_sum(total);
-    __syncwarp();
-    const int sub = lane % LANES, which = lane / LANES;
+    if (WARPS > 1) {
+        if (lane == 0) total_s[warp] = total;
+        __syncthreads();
+        total = (total_s[0] + total_s[1]) + (total_s[2] + total_s[3]);
+    } else {
+        __syncwarp();
+    }
+    const int sub = tid % LANES;
     float acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-    for (int c0 = which; c0 < parts; c0 += AT_ONCE * DEEP) {
+    for (int c0 = tid / LANES; c0 < parts; c0 += AT_ONCE * DEEP) {
         if constexpr (VEC) {
             float4 v[DEEP];
             float w[DEEP];
 #pragma unroll
             for (int k = 0; k < DEEP; ++k) {
                 const int c = c0 + k * AT_ONCE;
-                w[k] = c < parts ? weight_s[warp][c] : -1.0f;
-                v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (w[k] >= 0.0f || w[k] != w[k])
+                w[k] = c < parts ? weight_s[unit][c] : -1.0f;
+                if (w[k] != -1.0f)
                     v[k] = *reinterpret_cast<const float4*>(partial_acc + place(c) * d + 4 * sub);
             }
 #pragma unroll
@@ -214,7 +232,7 @@ shared_merge_kernel(T* __restrict__ out, int out_stride, const int* __restrict__
                 acc[3] = fmaf(w[k], v[k].w, acc[3]);
             }
         } else {
-            const float w = weight_s[warp][c0];
+            const float w = weight_s[unit][c0];
             if (w == -1.0f) continue;
             const size_t at = place(c0);
 #pragma unroll
@@ -228,22 +246,48 @@ shared_merge_kernel(T* __restrict__ out, int out_stride, const int* __restrict__
         for (int o = LANES; o < 32; o <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     T* dst = out + (size_t)token * out_stride + h * d;
-    if (which != 0) return;
+    if constexpr (WARPS == 1) {
+        if (tid >= LANES) return;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int f = VEC ? 4 * sub + i : sub + LANES * i;
-        if (f < d) dst[f] = from_float<T>(acc[i] * inv);
+        for (int i = 0; i < N; ++i) {
+            const int f = VEC ? 4 * sub + i : sub + LANES * i;
+            if (f < d) dst[f] = from_float<T>(acc[i] * inv);
+        }
+    } else {
+        if (lane < LANES) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int f = VEC ? 4 * sub + i : sub + LANES * i;
+                if (f < d) sum_s[warp][f] = acc[i];
+            }
+        }
+        __syncthreads();
+        for (int f = tid; f < d; f += GROUP)
+            dst[f] = from_float<T>(((sum_s[0][f] + sum_s[1][f]) + (sum_s[2][f] + sum_s[3][f])) * inv);
     }
 }
 
+// A warp alone reads up to MERGE_FEW results a row, four at once or eight; more are shared out over four
+// warps.  (us for all launches: 18 questions of 21 tokens behind two documents of 4,100 keys, where a row has
+// some ten results, 42.9 with a warp and 38.2 with four; 16 requests behind 4,096 keys, 32 heads of 64, 65
+// results, 25.2 and 14.4; 64 requests behind 16 prompts of 1,003 keys, five results, 55.5 and 57.5.)
+template <typename T, int WARPS>
+int merge_with(void* out, int out_stride, const int* token_seq, const int* seqs, const float* partial_acc,
+               const float* partial_ml, int tokens, int heads, int kv_heads, int d, cudaStream_t stream) {
+    const auto kernel = d == 128  ? shared_merge_kernel<T, WARPS, 32, true>
+                        : d == 64 ? shared_merge_kernel<T, WARPS, 16, true>
+                                  : shared_merge_kernel<T, WARPS, 32, false>;
+    const int units = 4 / WARPS;
+    return de_launch(kernel, dim3((unsigned)tokens, (heads + units - 1) / units), dim3(128), 0, stream,
+                     (T*)out, out_stride, token_seq, (const Joined*)seqs, partial_acc,
+                     (const float2*)partial_ml, heads, kv_heads, d);
+}
 template <typename T>
 int merge_of(void* out, int out_stride, const int* token_seq, const int* seqs, const float* partial_acc,
-             const float* partial_ml, int tokens, int heads, int kv_heads, int d, cudaStream_t stream) {
-    const auto kernel = d == 128  ? shared_merge_kernel<T, 32, true>
-                        : d == 64 ? shared_merge_kernel<T, 16, true>
-                                  : shared_merge_kernel<T, 32, false>;
-    return de_launch(kernel, dim3((unsigned)tokens, (heads + 3) / 4), dim3(128), 0, stream, (T*)out, out_stride, token_seq, (const Joined*)seqs, partial_acc,
-                     (const float2*)partial_ml, heads, kv_heads, d);
+             const float* partial_ml, int most, int tokens, int heads, int kv_heads, int d,
+             cudaStream_t stream) {
+    const auto f = most <= MERGE_FEW ? merge_with<T, 1> : merge_with<T, 4>;
+    return f(out, out_stride, token_seq, seqs, partial_acc, partial_ml, tokens, heads, kv_heads, d, stream);
 }
 
 template <typename T>
@@ -285,14 +329,15 @@ DE_EXPORT int de_shared_rows(int dtype, const void* q, int q_stride, const void*
              (cudaStream_t)stream);
 }
 
-// No row has more than de_shared_merge_most() partial results.
-DE_EXPORT int de_shared_merge_most() { return MERGE_MOST; }
+// `most`: partial results of a row, at most (up to 1,024).
 DE_EXPORT int de_shared_merge(int dtype, void* out, int out_stride, const int* token_seq,
                               const int* seqs, const float* partial_acc, const float* partial_ml,
-                              int tokens, int heads, int kv_heads, int head_dim, void* stream) {
+                              int most, int tokens, int heads, int kv_heads, int head_dim,
+                              void* stream) {
     if (tokens <= 0) return 0;
+    if (most < 0 || most > MERGE_MOST || heads > 262140) return -3;
     if (head_dim < 2 || head_dim > 256 || head_dim % 2 || kv_heads < 1 || heads % kv_heads) return -2;
     const auto f = dtype == DE_F32 ? merge_of<float> : merge_of<__nv_bfloat16>;
-    return f(out, out_stride, token_seq, seqs, partial_acc, partial_ml, tokens, heads, kv_heads, head_dim,
-             (cudaStream_t)stream);
+    return f(out, out_stride, token_seq, seqs, partial_acc, partial_ml, most, tokens, heads, kv_heads,
+             head_dim, (cudaStream_t)stream);
 }

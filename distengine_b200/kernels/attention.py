@@ -19,12 +19,11 @@ shares the batch.
 
 from __future__ import annotations
 
+import os
 from dataclasses import dataclass
 
 import numpy as np
 import torch
-
-import os
 
 from . import library
 from .attention_plan import build_plan, choose_chunk, choose_decode_split
@@ -34,7 +33,13 @@ MAX_HEAD_DIM = 256
 F32_CHUNK = 128          # keys in a chunk of the float32 path (a fixed order of summation)
 _status_fallback: "torch.Tensor | None" = None
 NARROW_ROWS = 16
-SHARED_SAVES = int(os.environ.get("SHARED_SAVES", 4 << 20))
+# Bytes of keys and values that a step must save by reading shared prefixes once before it goes through
+# the kernels for that, which are two or three launches more.  (us a layer, request by request and shared,
+# 32 heads.  bfloat16, 8 kv heads of 128: 8 x 8 behind 128 keys, 29 MB, 18.1 and 12.3; 16 behind 512, 31 MB,
+# 13.3 and 14.5; 4 behind 4,096, 50 MB, 33.1 and 13.3.  4 kv heads of 64: 4 x 4 behind 512, 6 MB, 8.3 and 9.1;
+# 64 behind 512, 33 MB, 11.0 and 13.4; 4 x 4 behind 8,192, 101 MB, 26.1 and 19.5.  float32, 8 kv heads of 128:
+# 4 behind 1,024, 25 MB, 21.7 and 26.4; 4 behind 2,048, 50 MB, 38.2 and 29.1.)
+SHARED_SAVES = 32 << 20
 
 
 def check_head_dim(head_dim: int) -> None:
@@ -195,7 +200,7 @@ class AttentionLauncher:
         prep.notes[self.key] = ()
         prep.notes[self.key + "/decode"] = None
         prep.notes[self.key + "/shared"] = (tuple(plan.shapes.items()), tuple(plan.items),
-                                            plan.partial_rows, plan.tokens)
+                                            plan.partial_rows, plan.most_parts, plan.tokens)
         return True
 
     def _prepare_decode(self, prep, force_split: "tuple[int, int, int] | None") -> None:
@@ -373,11 +378,11 @@ class AttentionLauncher:
                    v_pages: torch.Tensor, block_table: torch.Tensor, ctx) -> None:
         """A step of single tokens whose requests share prefixes; arguments as ``run``."""
         from .shared_prefix import SharedPlan
-        shapes, names, partial_rows, tokens = ctx.notes[self.key + "/shared"]
+        shapes, names, partial_rows, most_parts, tokens = ctx.notes[self.key + "/shared"]
         at = f"{self.key}/shared/"
         plan = SharedPlan({name: ctx.arrays[at + name] for name in names}, dict(shapes),
-                          ctx.arrays[at + "seqs"], ctx.arrays[at + "token_seq"], partial_rows, tokens,
-                          q.device)
+                          ctx.arrays[at + "seqs"], ctx.arrays[at + "token_seq"], partial_rows, most_parts,
+                          tokens, q.device)
         self.shared.run(q, out, k_pages, v_pages, block_table, ctx.seq_slot, ctx.seq_pos0, plan,
                         ctx.status, ctx.buffer)
 

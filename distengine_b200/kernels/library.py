@@ -161,7 +161,7 @@ SIGNATURES: dict[str, dict[str, list]] = {
     },
     "shared_prefix": {
         "de_shared_rows": [I, P, I, P, P, P, I, I, P, P, P, I, I, I, I, P, P, I, I, I, I, F, P, P],
-        "de_shared_merge_most": [], "de_shared_merge": [I, P, I, P, P, P, P, I, I, I, I, P],
+        "de_shared_merge": [I, P, I, P, P, P, P, I, I, I, I, I, P],
     },
     "shared_prefix_f32": {
         "de_shared_f32_unit": [], "de_shared_f32_held": [I, I],

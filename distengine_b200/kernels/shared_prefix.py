@@ -35,6 +35,7 @@ class SharedPlan:
     seqs: "np.ndarray | torch.Tensor"
     token_seq: "np.ndarray | torch.Tensor"
     partial_rows: int
+    most_parts: int          # partial results of a row, at most
     tokens: int
     device: "torch.device | None" = field(default=None)
 
@@ -42,7 +43,7 @@ class SharedPlan:
         move = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(device)
         seqs = move(self.seqs)
         return SharedPlan({name: move(a) for name, a in self.items.items()}, self.shapes, seqs,
-                          move(self.token_seq), self.partial_rows, self.tokens, seqs.device)
+                          move(self.token_seq), self.partial_rows, self.most_parts, self.tokens, seqs.device)
 
 
 @dataclass(frozen=True)
@@ -178,7 +179,8 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
     # (the tcgen05 kernel's blocks first: the others' fill the SMs that those leave)
     names = sorted(items, key=lambda name: (name != "tcgen05", name))
     return SharedPlan({name: np.concatenate(items[name]) for name in names}, shapes, seqs,
-                      np.repeat(np.arange(len(qlen)), qlen), base, total)
+                      np.repeat(np.arange(len(qlen)), qlen), base,
+                      int((seqs[:, 3] + seqs[:, 6]).max(initial=0)), total)
 
 
 class SharedPrefixAttention:
@@ -234,7 +236,7 @@ class SharedPrefixAttention:
             # 55.5 and 39.7; 20 rows behind 2,040 of 8 17.9 and 18.7; 37 rows behind 6,373 of 32 40.6 and,
             # three tiles, 44.2; 48 rows behind 1,214 of 4, head size 64, 16.0 and 12.5)
             if rows > 32 and wide:
-                return (Tile("tcgen05", 128, 128, sms, 2) if rows <= 128 else
+                return (Tile("tcgen05", 128, 128, sms, 2, least=256) if rows <= 128 else
                         Tile("tcgen05", 256, 128, sms))
             return few
 
@@ -321,5 +323,5 @@ class SharedPrefixAttention:
                        "shared prefix attention")
             behind = 1
         _check(lib.de_shared_merge(tag, out.data_ptr(), out.stride(0), plan.token_seq.data_ptr(),
-                                   plan.seqs.data_ptr(), acc.data_ptr(), ml.data_ptr(), tokens,
-                                   self.heads, self.kv_heads, d, _stream()), "shared prefix merge")
+                                   plan.seqs.data_ptr(), acc.data_ptr(), ml.data_ptr(), plan.most_parts,
+                                   tokens, self.heads, self.kv_heads, d, _stream()), "shared prefix merge")
