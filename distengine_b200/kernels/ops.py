@@ -774,17 +774,18 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, best: torch.Tensor, 
     then the lower token.  A total of minus infinity or NaN (a masked token, a dead beam, a row that
     holds NaN or plus infinity) is no candidate; where too few are left, best is minus infinity and
     beam and token are -1.  ``scratch``: uint8, ``beam_scratch`` bytes, used during the call."""
-    _need(logits.dim() == 2 and scores.dim() == 2 and best.dim() == 2,
+    _need(logits.dim() == scores.dim() == best.dim() == 2,
           "beam_select: logits [groups * beams, vocabulary], scores [groups, beams], best [groups, take]")
-    groups, beams = scores.shape
-    take, vocabulary = best.shape[1], logits.shape[1]
+    (rows, vocabulary), (stride, one) = logits.shape, logits.stride()
+    (groups, beams), taken = scores.shape, best.shape
+    take = taken[1]
     _need(logits.dtype == scores.dtype == best.dtype == torch.float32
           and beam.dtype == token.dtype == torch.int32,
           "beam_select: logits, scores and best are float32, beam and token int32")
-    _need(logits.shape[0] == groups * beams and best.shape == beam.shape == token.shape == (groups, take)
+    _need(rows == groups * beams and taken[0] == groups and taken == beam.shape == token.shape
           and scores.is_contiguous() and best.is_contiguous() and beam.is_contiguous()
-          and token.is_contiguous() and (vocabulary < 2 or logits.stride(1) == 1)
-          and (logits.shape[0] < 2 or logits.stride(0) >= vocabulary),
+          and token.is_contiguous() and (vocabulary < 2 or one == 1)
+          and (rows < 2 or stride >= vocabulary),
           "beam_select: a row of logits a beam; contiguous scores, best, beam and token")
     if not (1 <= beams <= MAX_BEAMS and 1 <= take <= MAX_TAKE and vocabulary >= 1):
         raise ValueError(f"beam_select: 1 to {MAX_BEAMS} beams, 1 to {MAX_TAKE} taken, a vocabulary; "
@@ -799,7 +800,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, best: torch.Tensor, 
           or scratch.device != logits.device or scratch.data_ptr() % 16):
         raise ValueError(f"beam_select: scratch must be {size} bytes (uint8), 16-byte aligned")
     lib = library.load("beam")
-    _check(lib.de_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), groups, beams,
+    _check(lib.de_beam_select(logits.data_ptr(), stride, scores.data_ptr(), groups, beams,
                               vocabulary, take, best.data_ptr(), beam.data_ptr(), token.data_ptr(),
                               scratch.data_ptr(), _stream()), "beam_select")
 

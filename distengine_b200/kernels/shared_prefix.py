@@ -268,60 +268,65 @@ class SharedPrefixAttention:
         first token, not before the prefix's end.  A token sees the keys up to its own position; a
         key without a page is not seen and sets ``status`` to 2.  ``buffer(name, shape, dtype)``:
         where the partial results lie during the call (None: fresh memory)."""
-        d, tokens = self.head_dim, plan.tokens
+        d, heads, kv_heads, tokens = self.head_dim, self.heads, self.kv_heads, plan.tokens
+        _need(q.dim() == out.dim() == 2, "shared prefix: q and out have a row a token of the plan")
+        _need(k_pages.dim() == 4, "shared prefix: pages must be [pages, kv_heads, page, head_dim]")
+        q_shape, (q_stride, q_one) = q.shape, q.stride()
+        out_shape, (out_stride, out_one) = out.shape, out.stride()
         _need(q.dtype == out.dtype == k_pages.dtype == v_pages.dtype == self.dtype,
               "shared prefix: q, out and the pages have the layer's dtype")
-        _need(q.dim() == 2 and out.dim() == 2 and q.stride(1) == 1 and out.stride(1) == 1
-              and q.shape[0] == out.shape[0] == tokens and q.shape[1] >= self.heads * d
-              and out.shape[1] == self.heads * d
-              and (tokens < 2 or (q.stride(0) >= self.heads * d and out.stride(0) >= self.heads * d)),
+        _need(q_one == 1 and out_one == 1 and q_shape[0] == out_shape[0] == tokens
+              and q_shape[1] >= out_shape[1] == heads * d
+              and (tokens < 2 or (q_stride >= heads * d and out_stride >= heads * d)),
               "shared prefix: q and out have a row a token of the plan, heads * d features each")
-        _need(k_pages.dim() == 4 and k_pages.is_contiguous() and v_pages.is_contiguous()
-              and k_pages.shape == v_pages.shape and k_pages.shape[1] == self.kv_heads
-              and k_pages.shape[3] == d and k_pages.shape[2] > 0,
+        pages, page_heads, page, page_dim = k_pages.shape
+        _need(k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.shape == v_pages.shape
+              and page_heads == kv_heads and page_dim == d and page > 0,
               "shared prefix: pages must be [pages, kv_heads, page, head_dim]")
-        for name, t in (("block_table", block_table), ("seq_slot", seq_slot), ("seq_pos0", seq_pos0)):
-            _need(t.dtype == torch.int32 and t.is_contiguous(),
-                  f"shared prefix: {name} must be a contiguous int32 tensor")
-        _need(block_table.dim() == 2 and seq_slot.shape == seq_pos0.shape == (plan.seqs.shape[0],),
+        _need(block_table.dtype == seq_slot.dtype == seq_pos0.dtype == torch.int32
+              and block_table.is_contiguous() and seq_slot.is_contiguous() and seq_pos0.is_contiguous(),
+              "shared prefix: block_table, seq_slot and seq_pos0 must be contiguous int32 tensors")
+        _need(block_table.dim() == 2 and seq_slot.shape == seq_pos0.shape == plan.seqs.shape[:1],
               "shared prefix: block_table [slots, pages], a slot and a position a request")
         _need(plan.device is not None, "shared prefix: the plan is not on the device yet (plan.to)")
         _on_device(q, out, k_pages, v_pages, block_table, seq_slot, seq_pos0, plan.seqs)
         if tokens == 0:
             return
         status = _status_word(status, q)
-        make = buffer or (lambda name, shape, dtype: torch.empty(shape, dtype=dtype, device=q.device))
-        rows = plan.partial_rows * self.kv_heads
-        acc = make("shared_prefix.partial_acc", (rows * d,), torch.float32)
-        ml = make("shared_prefix.partial_ml", (rows * 2,), torch.float32)
+        # sums and, behind them, the maximum and the sum of weights of every partial result
+        rows = plan.partial_rows * kv_heads
+        shape = (rows * (d + 2),)
+        partial = (torch.empty(shape, dtype=torch.float32, device=q.device) if buffer is None else
+                   buffer("shared_prefix.partial", shape, torch.float32))
+        acc = partial.data_ptr()
+        ml = acc + 4 * rows * d
         lib = library.load("shared_prefix")
-        tag = _tag(q.dtype)
+        tag, stream = _tag(self.dtype), _stream()
+        q_at, k_at, v_at = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
         # what a kernel copies in pieces has to lie so; the next one in this list takes it otherwise
-        pages_fit = not (k_pages.data_ptr() % 16 or v_pages.data_ptr() % 16)
-        aligned = pages_fit and not (q.stride(0) % 2 or q.data_ptr() % 4)
-        wide = pages_fit and not (q.stride(0) % 8 or q.data_ptr() % 16)
+        pages_fit = not (k_at % 16 or v_at % 16)
+        aligned = pages_fit and not (q_stride % 2 or q_at % 4)
+        wide = pages_fit and not (q_stride % 8 or q_at % 16)
+        before = (q_at, q_stride, k_at, v_at, block_table.data_ptr(), block_table.stride(0), pages,
+                  seq_slot.data_ptr(), seq_pos0.data_ptr())
+        after = (acc, ml, heads, kv_heads, d, page, self.scale, status.data_ptr(), stream)
         behind = 0
         for name, items in plan.items.items():
             rows, unit = plan.shapes[name]
-            before = (q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
-                      block_table.data_ptr(), block_table.stride(0), k_pages.shape[0],
-                      seq_slot.data_ptr(), seq_pos0.data_ptr(), items.data_ptr(), items.shape[0])
-            after = (acc.data_ptr(), ml.data_ptr(), self.heads, self.kv_heads, d, k_pages.shape[2],
-                     self.scale, status.data_ptr(), _stream())
+            work = (*before, items.data_ptr(), items.shape[0])
             if (name == "tcgen05" and wide and not behind
-                    and (kernel := library.load(*self.tcgen05_module)).de_shared_tcgen05_page_ok(
-                        k_pages.shape[2])):
-                _check(kernel.de_shared_tcgen05(*before, *after), "shared prefix attention (tcgen05)")
+                    and (kernel := library.load(*self.tcgen05_module)).de_shared_tcgen05_page_ok(page)):
+                _check(kernel.de_shared_tcgen05(*work, *after), "shared prefix attention (tcgen05)")
             elif name.startswith("f32") and pages_fit:
-                _check(library.load("shared_prefix_f32").de_shared_f32(*before, rows, behind, *after),
+                _check(library.load("shared_prefix_f32").de_shared_f32(*work, rows, behind, *after),
                        "shared prefix attention (float32)")
             elif name in ("warp", "tcgen05") and aligned:
-                _check(library.load(*self.mma_module).de_shared_mma(*before, rows, behind, *after),
+                _check(library.load(*self.mma_module).de_shared_mma(*work, rows, behind, *after),
                        "shared prefix attention (mma)")
             else:
-                _check(lib.de_shared_rows(tag, *before, rows, unit, behind, *after),
+                _check(lib.de_shared_rows(tag, *work, rows, unit, behind, *after),
                        "shared prefix attention")
             behind = 1
-        _check(lib.de_shared_merge(tag, out.data_ptr(), out.stride(0), plan.token_seq.data_ptr(),
-                                   plan.seqs.data_ptr(), acc.data_ptr(), ml.data_ptr(), plan.most_parts,
-                                   tokens, self.heads, self.kv_heads, d, _stream()), "shared prefix merge")
+        _check(lib.de_shared_merge(tag, out.data_ptr(), out_stride, plan.token_seq.data_ptr(),
+                                   plan.seqs.data_ptr(), acc, ml, plan.most_parts, tokens, heads,
+                                   kv_heads, d, stream), "shared prefix merge")
