@@ -38,7 +38,7 @@ shared_rows_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ 
                    int table_stride, int num_pages, const int* __restrict__ seq_slot,
                    const int* __restrict__ seq_pos0, const Item* __restrict__ items,
                    float* __restrict__ partial_acc, float2* __restrict__ partial_ml, int heads,
-                   int kv_heads, int d, int page, float scale, int unit, int behind,
+                   int kv_heads, int d, int page, float scale, int unit, int order,
                    int* __restrict__ status) {
     extern __shared__ float smem[];
     const int ld = d + 1;
@@ -50,7 +50,9 @@ shared_rows_kernel(const T* __restrict__ q, int q_stride, const T* __restrict__ 
     const int hk = blockIdx.x % kv_heads, g = heads / kv_heads;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int first = blockIdx.y * ROWS;                  // of the tile's rows
+    const bool behind = order & BEHIND;
     if (!behind) pdl_wait();
+    if (order & FOLLOWED) pdl_trigger();
     if (first >= it.count) {
         if (behind) pdl_wait();
         return;
@@ -294,7 +296,7 @@ template <typename T>
 int rows_of(const void* q, int q_stride, const void* k_pages, const void* v_pages,
             const int* block_table, int table_stride, int num_pages, const int* seq_slot,
             const int* seq_pos0, const int* items, int num_items, int tile_rows, int unit,
-            int behind, float* partial_acc, float* partial_ml, int heads, int kv_heads, int d, int page,
+            int order, float* partial_acc, float* partial_ml, int heads, int kv_heads, int d, int page,
             float scale, int* status, cudaStream_t stream) {
     const int smem = (ROWS * d + 2 * KT * (d + 1)) * 4;
     if (smem > 40 * 1024) {
@@ -305,18 +307,18 @@ int rows_of(const void* q, int q_stride, const void* k_pages, const void* v_page
     return de_launch(shared_rows_kernel<T>, dim3((unsigned)num_items * kv_heads, (tile_rows + ROWS - 1) / ROWS),
                      dim3(THREADS), smem, stream, (const T*)q, q_stride, (const T*)k_pages, (const T*)v_pages, block_table,
                      table_stride, num_pages, seq_slot, seq_pos0, (const Item*)items, partial_acc,
-                     (float2*)partial_ml, heads, kv_heads, d, page, scale, unit, behind, status);
+                     (float2*)partial_ml, heads, kv_heads, d, page, scale, unit, order, status);
 }
 
 }  // namespace
 
-// `tile_rows`: most rows of an item; `unit`: what the ranges of own keys are a multiple of; `behind`:
-// the launch before this one is another of the same step's (see shared_prefix.cuh).
+// `tile_rows`: most rows of an item; `unit`: what the ranges of own keys are a multiple of; `order`:
+// 1 where the launch before this one is another of the same step's, 2 where the next one is.
 DE_EXPORT int de_shared_rows(int dtype, const void* q, int q_stride, const void* k_pages,
                              const void* v_pages, const int* block_table, int table_stride,
                              int num_pages, const int* seq_slot, const int* seq_pos0,
                              const int* items, int num_items, int tile_rows, int unit,
-                             int behind, float* partial_acc, float* partial_ml, int heads, int kv_heads,
+                             int order, float* partial_acc, float* partial_ml, int heads, int kv_heads,
                              int head_dim, int page, float scale, int* status, void* stream) {
     if (num_items <= 0) return 0;
     if (tile_rows < 1 || tile_rows > 1024 || unit < 1) return -3;
@@ -325,7 +327,7 @@ DE_EXPORT int de_shared_rows(int dtype, const void* q, int q_stride, const void*
         return -2;
     const auto f = dtype == DE_F32 ? rows_of<float> : rows_of<__nv_bfloat16>;
     return f(q, q_stride, k_pages, v_pages, block_table, table_stride, num_pages, seq_slot, seq_pos0,
-             items, num_items, tile_rows, unit, behind, partial_acc, partial_ml, heads, kv_heads, head_dim, page, scale, status,
+             items, num_items, tile_rows, unit, order, partial_acc, partial_ml, heads, kv_heads, head_dim, page, scale, status,
              (cudaStream_t)stream);
 }
 

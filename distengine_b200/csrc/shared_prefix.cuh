@@ -4,12 +4,16 @@
 
 #include "common.cuh"
 
-// The kernels of a step do not depend on one another, and each lets its successor start once its own
-// wait for its predecessor has returned.  So those behind the first (`behind`) need not wait before they
-// begin: what the step reads was complete when the first one's wait returned.  They wait before they
-// end instead, so that what waits for them has waited for all.
+// The kernels of a step do not depend on one another, so one that another of them follows lets it start at
+// once (FOLLOWED), on the SMs' memory and slots that its own blocks leave; the last one lets the merge
+// start when it is nearly done.  Those behind the first (BEHIND) need not wait before they begin: the first
+// one's blocks let them start after their own wait, when what the step reads was complete.  They wait
+// before they end instead, so that what waits for them has waited for all.  (Started when the one before
+// ends, the second kernel of eight beams in float32 made 25.2 us of 14.8.)
 
 namespace shared_prefix {
+
+constexpr int BEHIND = 1, FOLLOWED = 2;                   // bits of `order`
 
 constexpr int HALF_ROWS = 128;
 

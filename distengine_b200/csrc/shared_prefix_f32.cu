@@ -41,7 +41,7 @@ shared_f32_kernel(const float* __restrict__ q, int q_stride, const float* __rest
                   int table_stride, int num_pages, const int* __restrict__ seq_slot,
                   const int* __restrict__ seq_pos0, const Item* __restrict__ items,
                   float* __restrict__ partial_acc, float2* __restrict__ partial_ml, int heads,
-                  int kv_heads, int d, int page, float scale, int behind, int* __restrict__ status) {
+                  int kv_heads, int d, int page, float scale, int order, int* __restrict__ status) {
     constexpr int ROWS = 8 * RPT, GROUPS = DMAX / 64, PS = weight_stride<RPT>();
     extern __shared__ __align__(16) float smem[];
     float* q_s = smem;                                    // [ROWS][d]
@@ -52,7 +52,9 @@ shared_f32_kernel(const float* __restrict__ q, int q_stride, const float* __rest
     const Item it = items[blockIdx.x / kv_heads];
     const int hk = blockIdx.x % kv_heads, g = heads / kv_heads;
     const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;
+    const bool behind = order & BEHIND;
     if (!behind) pdl_wait();
+    if (order & FOLLOWED) pdl_trigger();
     const Range range = range_of(it, seq_pos0, g, KT);
     const int slot = seq_slot[it.seq];
     const int tiles = (range.end - range.begin + KT - 1) / KT;
@@ -240,7 +242,7 @@ shared_f32_kernel(const float* __restrict__ q, int q_stride, const float* __rest
 template <int DMAX, int RPT>
 int launch(const float* q, int q_stride, const float* k_pages, const float* v_pages,
            const int* block_table, int table_stride, int num_pages, const int* seq_slot,
-           const int* seq_pos0, const int* items, int num_items, int behind, float* partial_acc,
+           const int* seq_pos0, const int* items, int num_items, int order, float* partial_acc,
            float* partial_ml, int heads, int kv_heads, int d, int page, float scale, int* status,
            cudaStream_t stream) {
     const int smem = smem_floats<RPT>(d) * 4;
@@ -252,7 +254,7 @@ int launch(const float* q, int q_stride, const float* k_pages, const float* v_pa
     return de_launch(shared_f32_kernel<DMAX, RPT>, dim3((unsigned)num_items * kv_heads), dim3(THREADS),
                      smem, stream, q, q_stride, k_pages, v_pages, block_table, table_stride, num_pages,
                      seq_slot, seq_pos0, (const Item*)items, partial_acc, (float2*)partial_ml, heads,
-                     kv_heads, d, page, scale, behind, status);
+                     kv_heads, d, page, scale, order, status);
 }
 
 }  // namespace
@@ -267,11 +269,11 @@ DE_EXPORT int de_shared_f32_held(int rows, int head_dim) {
     return blocks > 6 ? 6 : blocks;
 }
 
-// Items of up to `rows` rows; pages in 16-byte pieces; `behind` as in shared_prefix.cu.
+// Items of up to `rows` rows; pages in 16-byte pieces; `order` as in shared_prefix.cu.
 DE_EXPORT int de_shared_f32(const float* q, int q_stride, const float* k_pages, const float* v_pages,
                             const int* block_table, int table_stride, int num_pages,
                             const int* seq_slot, const int* seq_pos0, const int* items, int num_items,
-                            int rows, int behind, float* partial_acc, float* partial_ml, int heads,
+                            int rows, int order, float* partial_acc, float* partial_ml, int heads,
                             int kv_heads, int head_dim, int page, float scale, int* status,
                             void* stream) {
     if (num_items <= 0) return 0;
@@ -284,6 +286,6 @@ DE_EXPORT int de_shared_f32(const float* q, int q_stride, const float* k_pages, 
                    : rows == 16 ? (sizes == 0 ? launch<64, 2> : sizes == 1 ? launch<128, 2> : launch<256, 2>)
                                 : (sizes == 0 ? launch<64, 4> : sizes == 1 ? launch<128, 4> : launch<256, 4>);
     return f(q, q_stride, k_pages, v_pages, block_table, table_stride, num_pages, seq_slot, seq_pos0, items,
-             num_items, behind, partial_acc, partial_ml, heads, kv_heads, head_dim, page, scale, status,
+             num_items, order, partial_acc, partial_ml, heads, kv_heads, head_dim, page, scale, status,
              (cudaStream_t)stream);
 }

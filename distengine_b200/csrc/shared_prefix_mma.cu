@@ -45,11 +45,12 @@ shared_mma_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
                   int table_stride, int num_pages, const int* __restrict__ seq_slot,
                   const int* __restrict__ seq_pos0, const Item* __restrict__ items, int num_items,
                   float* __restrict__ partial_acc, float2* __restrict__ partial_ml, int heads,
-                  int kv_heads, int page, float scale, int behind, int* __restrict__ status) {
+                  int kv_heads, int page, float scale, int order, int* __restrict__ status) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int gid = lane >> 2, tig = lane & 3;
     const int g = heads / kv_heads;
+    const bool behind = order & BEHIND;
     const long long place = (long long)blockIdx.x * WARPS + warp;
     if (place >= (long long)num_items * kv_heads) {       // (a warp of the last block)
         pdl_wait();
@@ -60,6 +61,7 @@ shared_mma_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
     __nv_bfloat16* ring = reinterpret_cast<__nv_bfloat16*>(smem_raw) + warp * STAGES * STAGE;
     const bool second = has_second_place(it);
     if (!behind) pdl_wait();
+    if (order & FOLLOWED) pdl_trigger();
     const Range range = range_of(it, seq_pos0, g, NK);
     // of an item with more rows than a warp takes, the warp's
     it.row0 += blockIdx.y * ROWS;
@@ -284,12 +286,12 @@ DE_EXPORT int de_shared_mma_rows() { return ROWS; }
 DE_EXPORT int de_shared_mma_unit() { return NK; }
 DE_EXPORT int de_shared_mma_held() { return BLOCKS * WARPS; }
 
-// `tile_rows`: most rows of an item (above de_shared_mma_rows() several warps'); `behind` as in
+// `tile_rows`: most rows of an item (above de_shared_mma_rows() several warps'); `order` as in
 // shared_prefix.cu; q in 4-byte pieces, pages in 16-byte ones.
 DE_EXPORT int de_shared_mma(const void* q, int q_stride, const void* k_pages, const void* v_pages,
                             const int* block_table, int table_stride, int num_pages,
                             const int* seq_slot, const int* seq_pos0, const int* items, int num_items,
-                            int tile_rows, int behind, float* partial_acc, float* partial_ml, int heads,
+                            int tile_rows, int order, float* partial_acc, float* partial_ml, int heads,
                             int kv_heads, int head_dim, int page, float scale, int* status,
                             void* stream) {
     if (num_items <= 0) return 0;
@@ -310,5 +312,5 @@ DE_EXPORT int de_shared_mma(const void* q, int q_stride, const void* k_pages, co
                      (const __nv_bfloat16*)q, q_stride, (const __nv_bfloat16*)k_pages,
                      (const __nv_bfloat16*)v_pages, block_table, table_stride, num_pages, seq_slot,
                      seq_pos0, (const Item*)items, num_items, partial_acc, (float2*)partial_ml, heads,
-                     kv_heads, page, scale, behind, status);
+                     kv_heads, page, scale, order, status);
 }

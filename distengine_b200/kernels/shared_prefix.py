@@ -310,23 +310,23 @@ class SharedPrefixAttention:
         before = (q_at, q_stride, k_at, v_at, block_table.data_ptr(), block_table.stride(0), pages,
                   seq_slot.data_ptr(), seq_pos0.data_ptr())
         after = (acc, ml, heads, kv_heads, d, page, self.scale, status.data_ptr(), stream)
-        behind = 0
-        for name, items in plan.items.items():
+        last = len(plan.items) - 1
+        for i, (name, items) in enumerate(plan.items.items()):
+            order = (i > 0) + 2 * (i < last)              # behind another kernel, followed by one
             rows, unit = plan.shapes[name]
             work = (*before, items.data_ptr(), items.shape[0])
-            if (name == "tcgen05" and wide and not behind
+            if (name == "tcgen05" and wide and not i
                     and (kernel := library.load(*self.tcgen05_module)).de_shared_tcgen05_page_ok(page)):
                 _check(kernel.de_shared_tcgen05(*work, *after), "shared prefix attention (tcgen05)")
             elif name.startswith("f32") and pages_fit:
-                _check(library.load("shared_prefix_f32").de_shared_f32(*work, rows, behind, *after),
+                _check(library.load("shared_prefix_f32").de_shared_f32(*work, rows, order, *after),
                        "shared prefix attention (float32)")
             elif name in ("warp", "tcgen05") and aligned:
-                _check(library.load(*self.mma_module).de_shared_mma(*work, rows, behind, *after),
+                _check(library.load(*self.mma_module).de_shared_mma(*work, rows, order, *after),
                        "shared prefix attention (mma)")
             else:
-                _check(lib.de_shared_rows(tag, *work, rows, unit, behind, *after),
+                _check(lib.de_shared_rows(tag, *work, rows, unit, order, *after),
                        "shared prefix attention")
-            behind = 1
         _check(lib.de_shared_merge(tag, out.data_ptr(), out_stride, plan.token_seq.data_ptr(),
                                    plan.seqs.data_ptr(), acc, ml, plan.most_parts, tokens, heads,
                                    kv_heads, d, stream), "shared prefix merge")
