@@ -80,6 +80,20 @@ __device__ __forceinline__ bool wait(void* bar, unsigned parity, int* status) {
     atomicExch(status, 3);
     return false;
 }
+__device__ __forceinline__ void store_release(int* at, int v) {
+    asm volatile("st.release.cta.shared::cta.s32 [%0], %1;\n" ::"r"(smem_u32(at)), "r"(v) : "memory");
+}
+// Bounded wait for a number above n.
+__device__ __forceinline__ bool wait_above(int* at, int n, int* status) {
+    for (unsigned spins = 0; spins < SPIN_LIMIT; ++spins) {
+        int v;
+        asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];\n" : "=r"(v) : "r"(smem_u32(at)) : "memory");
+        if (v > n) return true;
+        if (spins > 8) __nanosleep(100);
+    }
+    atomicExch(status, 3);
+    return false;
+}
 // The products and their commits are issued by a whole warp, of which one elected thread (the same every
 // time) takes effect: so the operands are known to be the same in all lanes.  Behind a branch on the lane
 // an instruction takes 160 cycles to issue, eight of 128 x 128 x 16 1,307 instead of their 514.
@@ -223,10 +237,11 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
     unsigned long long* p_ready = s_done + 2;             // [2] weights are written (256 arrivals)
     unsigned long long* o_done = s_done + 4;              // [2] weights times values is complete
     unsigned long long* s_free = s_done + 6;              // [2] scores are in registers (256 arrivals)
-    unsigned long long* drained = s_done + 8;             // [2] what is issued is complete, after a failed wait
+    unsigned long long* drained = s_done + 8;             // [2] what is issued is complete
     unsigned long long* p_half = s_done + 10;             // [2] those of the first 64 keys are
     unsigned& tmem_slot = *reinterpret_cast<unsigned*>(s_done + 12);
     int& missing_s = *reinterpret_cast<int*>(s_done + 13);
+    int* issued_s = &missing_s + 1;                       // units whose copies have begun
     float* exchange = reinterpret_cast<float*>(ring + BUFFERS * BUFFER + 512);   // [pipeline][half][row]
 
     const Item it = items[blockIdx.x / kv_heads];
@@ -243,6 +258,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
 
     if (tid == 0) {
         missing_s = 0;
+        *issued_s = 0;
         mbar_init(&drained[0], 1);
         mbar_init(&drained[1], 1);
         for (int i = 0; i < BUFFERS; ++i) {
@@ -306,6 +322,14 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
     const unsigned tmem = tmem_slot;
     const bool missing = missing_s != 0;
     bool ok = aligned;
+    // Waits until unit `u` (keys of tile u / 2, or its values) has landed.  A barrier's wait tells a phase
+    // from its neighbours only.  Where the pipelines take turns the last unit in the buffer was the other
+    // one's and may still be on its way although later ones have landed; so it is first made sure that the
+    // copies of `u` have begun, before which that one has landed and been read.
+    auto landed = [&](int u) {
+        if (turns && ok) ok = wait_above(issued_s, u, status);
+        if (ok) ok = wait(&full[u % BUFFERS], (u / BUFFERS) & 1, status);
+    };
 
     if (warp == COPY_WARP) {
         // ------------------------------------------------------------------ copies
@@ -324,7 +348,10 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
                 if (unit >= BUFFERS && ok) ok = wait(&empty[b], (unit / BUFFERS - 1) & 1, status);
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 if (!ok) break;
-                if (lane == 0) mbar_expect_tx(&full[b], bytes);
+                if (lane == 0) {
+                    mbar_expect_tx(&full[b], bytes);
+                    store_release(issued_s, unit + 1);
+                }
                 ++issued;
                 __syncwarp();
                 if (id >= 0)
@@ -352,7 +379,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         // (a buffer's wait first: it is over long before the other one nearly always)
         auto scores = [&](int j, void* bar, unsigned parity) {
             const int unit = 2 * tile_of(i, j), b = unit % BUFFERS;
-            if (ok) ok = wait(&full[b], (unit / BUFFERS) & 1, status);
+            landed(unit);
             if (!passed(bar, parity)) return;
 #pragma unroll
             for (int sub = 0; sub < KS; ++sub) {
@@ -370,7 +397,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             if (!OVER && j + 1 < n) scores(j + 1, &s_free[i], j & 1);     // once these are in registers
             const int unit = 2 * tile_of(i, j) + 1, b = unit % BUFFERS;
             const unsigned long long vb = value_desc(ring + b * BUFFER);
-            if (ok) ok = wait(&full[b], (unit / BUFFERS) & 1, status);
+            landed(unit);
             if (!passed(&p_half[i], j & 1)) break;
 #pragma unroll
             for (int k = 0; k < KT / 32; ++k)
@@ -385,10 +412,9 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             commit(&empty[b]);
             if (OVER && j + 1 < n) scores(j + 1, &o_done[i], j & 1);      // the weights lie where they will
         }
-        if (!ok) {                    // what is issued ends before the tensor memory is freed
-            commit(&drained[i]);
-            wait(&drained[i], 0, status);
-        }
+        // what is issued, the last buffers' commits with it, ends before the block does
+        commit(&drained[i]);
+        wait(&drained[i], 0, status);
         __syncwarp();
     } else {
         // ------------------------------------------------------------------ softmax
@@ -406,6 +432,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             constexpr bool EDGE = decltype(edge)::value;
             const int t = tile_of(x, j), kt = it.begin + t * KT;
             if (ok) ok = wait(&s_done[x], j & 1, status);
+            __syncwarp();
             after_sync();
             unsigned sv[2][32];
             tmem_load_32cols(s_addr, sv[0]);
@@ -443,6 +470,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             if (any_of_pair(pair, (m - m_ref) * sl > RAISE)) {
                 if (!rest) {
                     if (ok) ok = wait(&o_done[x], (j - 1) & 1, status);
+                    __syncwarp();
                     after_sync();
                     rest = true;
                 }
@@ -473,6 +501,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             const Two sl2 = two(sl, sl), off2 = two(off, off);
             if (!rest) {                                  // the weights' columns are free
                 if (ok) ok = wait(&o_done[x], (j - 1) & 1, status);
+                __syncwarp();
                 after_sync();
             }
             Two sum2[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
@@ -495,7 +524,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
                     // first thread of row i has the values of key i (both pipelines write the same zeros).
                     if (EDGE && half == 0 && (kt + rowi >= it.end || (gone >> (rowi / box) & 1))) {
                         const int unit = 2 * t + 1, b = unit % BUFFERS;
-                        if (ok) ok = wait(&full[b], (unit / BUFFERS) & 1, status);
+                        landed(unit);
 #pragma unroll
                         for (int sub = 0; sub < KS; ++sub) {
                             uint4* v = reinterpret_cast<uint4*>(ring + b * BUFFER + sub * SUB + rowi * 128);
@@ -504,6 +533,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
                         }
                         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     }
+                    if constexpr (EDGE) __syncwarp();
                     tmem_wait_stores();
                     before_sync();
                     mbar_arrive(&p_half[x]);
@@ -524,6 +554,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         }
         if (n_of[x] > 0) {
             if (ok) ok = wait(&o_done[x], (n_of[x] - 1) & 1, status);
+            __syncwarp();
             after_sync();
         }
         // The rows' results go out by way of the ring (which nobody reads any more when both pipelines

@@ -328,3 +328,16 @@ def test_offsets_beyond_32_bits():
         want, tol = case.want()
         assert bool(((out.double().cpu().view_as(want) - want).abs() <= tol).all())
         del big
+
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("d", [64, 128])
+def test_pipelines_that_take_turns(page, d):
+    """Up to 128 rows a block's two pipelines take the tiles of keys in turn, so a buffer that the one has
+    read is filled for the other: which must not take what lay there before for its own, however late
+    that one landed.  The same bits every time, whatever the caches hold."""
+    case = Case([(12000, [(3, 1)] * 9)], 32, 8, d, page, torch.bfloat16, seed=page + d)
+    first = case.check(tail=4)
+    for _ in range(8):
+        torch.zeros(1 << 28, device=DEV)
+        assert torch.equal(case.run(tail=4), first)
