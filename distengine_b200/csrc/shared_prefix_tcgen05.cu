@@ -12,7 +12,7 @@
 //     bfloat16 back into tensor memory as the A operand of the second product;
 //   * warps 16 and 17, one thread each, issue a pipeline's s = q k^T (operands in shared memory) and
 //     o += p v (p in tensor memory, v MN-major straight from the pages);
-//   * warp 18 fetches: a ring of buffers of 128 keys or 128 values, one TMA box a page and 64 features.
+//   * warp 18 (and 19) fetch: a ring of buffers of 128 keys or 128 values, one TMA box a page and 64 features.
 // A row's exponentials refer to a maximum that is raised, and o rescaled, only when a score has grown by
 // more than 2^8 beyond it.
 //
@@ -49,7 +49,11 @@ constexpr int SUB = 128 * 128;                // bytes of a sub-tile: 128 rows o
 constexpr int BUFFER = KS * SUB;              // 128 keys, or their values
 constexpr int BUFFERS = D == 64 ? 10 : 5;     // what shared memory has room for beside q
 constexpr int SOFTMAX_WARPS = 16, MMA_WARP = 16, COPY_WARP = 18;
-constexpr int THREADS = 19 * 32;
+// Where the pipelines take turns, two warps fetch: one issues a box in some 100 cycles, too slowly for small
+// pages (108 rows behind 15,566 keys in pages of 16: 92 us, with two 77; in pages of 128 83 and 71).
+// Elsewhere one keeps up (512 rows behind 65,003 keys: 170 us, with two 178).
+template <bool TURNS> __host__ __device__ constexpr int copy_warps() { return TURNS ? 2 : 1; }
+template <bool TURNS> __host__ __device__ constexpr int threads() { return (COPY_WARP + copy_warps<TURNS>()) * 32; }
 constexpr int SMEM = 2 * BUFFER + BUFFERS * BUFFER + 512 + 2 * 2 * LANES * 4;
 constexpr int COLUMNS = 512;
 // columns of tensor memory: scores of pipeline x at 128 x; results at 256 + D x; weights (64 columns) over
@@ -219,7 +223,9 @@ template <bool B> struct Truth {
     static constexpr bool value = B;
 };
 
-__global__ void __launch_bounds__(THREADS, 1)
+// TURNS: there are items of up to 128 rows, whose tiles the pipelines take in turn
+template <bool TURNS>
+__global__ void __launch_bounds__(threads<TURNS>(), 1)
 shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
                       const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const int* __restrict__ block_table,
@@ -247,7 +253,8 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
     const Item it = items[blockIdx.x / kv_heads];
     const int hk = blockIdx.x % kv_heads, g = heads / kv_heads;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const bool turns = it.split != 0;                     // the pipelines take the tiles in turn
+    const bool turns = TURNS && it.split != 0;            // the pipelines take the tiles in turn
+    constexpr int THREADS = threads<TURNS>(), COPIERS = copy_warps<TURNS>();
     const int n_tiles = (it.end - it.begin + KT - 1) / KT;
     const bool aligned = (smem_u32(smem_raw) & 1023u) == 0;
     if (!aligned && tid == 0) atomicExch(status, 4);
@@ -262,7 +269,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         mbar_init(&drained[0], 1);
         mbar_init(&drained[1], 1);
         for (int i = 0; i < BUFFERS; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], COPIERS);
             mbar_init(&empty[i], !turns && it.count > LANES ? 2 : 1);      // pipelines that read it
         }
         for (int x = 0; x < 2; ++x) {
@@ -331,14 +338,15 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         if (ok) ok = wait(&full[u % BUFFERS], (u / BUFFERS) & 1, status);
     };
 
-    if (warp == COPY_WARP) {
+    if (warp >= COPY_WARP) {
         // ------------------------------------------------------------------ copies
-        // unit 2 t: the keys of tile t, unit 2 t + 1: its values
+        // unit 2 t: the keys of tile t, unit 2 t + 1: its values; the warps take the boxes in turn
+        const int w = warp - COPY_WARP, i = COPIERS * lane + w;
         int issued = 0;
         for (int t = 0; t < n_tiles; ++t) {
-            const int key = it.begin + t * KT + lane * box;
+            const int key = it.begin + t * KT + i * box;
             int id = -1;
-            if (lane < boxes && key < it.end) id = page_at(key);
+            if (i < boxes && key < it.end) id = page_at(key);
             const unsigned there = __ballot_sync(0xffffffffu, id >= 0);
             const unsigned bytes = __popc(there) * (unsigned)(box * 128 * KS);
             const int y = (int)((((long long)id * kv_heads + hk) * page + key % page));
@@ -350,14 +358,14 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
                 if (!ok) break;
                 if (lane == 0) {
                     mbar_expect_tx(&full[b], bytes);
-                    store_release(issued_s, unit + 1);
+                    if (TURNS && w == 0) store_release(issued_s, unit + 1);
                 }
                 ++issued;
                 __syncwarp();
                 if (id >= 0)
 #pragma unroll
                     for (int sub = 0; sub < KS; ++sub)
-                        tma_load_2d(ring + b * BUFFER + sub * SUB + lane * box * 128, v ? &map_v : &map_k,
+                        tma_load_2d(ring + b * BUFFER + sub * SUB + i * box * 128, v ? &map_v : &map_k,
                                     &full[b], 64 * sub, y);
             }
             if (!ok) break;
@@ -599,11 +607,11 @@ DE_EXPORT int de_shared_tcgen05_page_ok(int page) {
     return page >= 8 && page % 8 == 0 && (KT % page == 0 || page % KT == 0);
 }
 
-// Items of shared keys; q, pages in 16-byte pieces.
+// Items of shared keys; q, pages in 16-byte pieces.  `turns`: some have two places.
 DE_EXPORT int de_shared_tcgen05(const void* q, int q_stride, const void* k_pages, const void* v_pages,
                                 const int* block_table, int table_stride, int num_pages,
                                 const int* seq_slot, const int* seq_pos0, const int* items,
-                                int num_items, float* partial_acc, float* partial_ml, int heads,
+                                int num_items, int turns, float* partial_acc, float* partial_ml, int heads,
                                 int kv_heads, int head_dim, int page, float scale, int* status,
                                 void* stream) {
     (void)seq_pos0;
@@ -620,11 +628,12 @@ DE_EXPORT int de_shared_tcgen05(const void* q, int q_stride, const void* k_pages
     if (code) return code;
     code = tensor_maps::make(&map_v, v_pages, rows, D, D, page < KT ? page : KT, 64);
     if (code) return code;
-    const cudaError_t e = cudaFuncSetAttribute(shared_tcgen05_kernel,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    const auto kernel = turns ? shared_tcgen05_kernel<true> : shared_tcgen05_kernel<false>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return (int)e;
-    return de_launch(shared_tcgen05_kernel, dim3((unsigned)num_items * kv_heads), dim3(THREADS), SMEM,
-                     (cudaStream_t)stream, (const __nv_bfloat16*)q, q_stride, map_k, map_v, block_table,
-                     table_stride, num_pages, seq_slot, (const Item*)items, partial_acc,
-                     (float2*)partial_ml, heads, kv_heads, page, scale, status);
+    return de_launch(kernel, dim3((unsigned)num_items * kv_heads),
+                     dim3(turns ? threads<true>() : threads<false>()), SMEM, (cudaStream_t)stream,
+                     (const __nv_bfloat16*)q, q_stride, map_k, map_v, block_table, table_stride, num_pages,
+                     seq_slot, (const Item*)items, partial_acc, (float2*)partial_ml, heads, kv_heads, page,
+                     scale, status);
 }

@@ -27,23 +27,27 @@ MAX_SPLITS = 256         # ranges that a prefix or a request's own keys are cut 
 
 @dataclass
 class SharedPlan:
-    """The work lists of a step's requests: ``items`` by kernel, int32 [n, 8] (``shared_prefix::
-    Item``; ``shapes``: their most rows and the unit of their ranges), ``seqs`` int32 [requests, 8] (``shared_prefix::Joined``), ``token_seq`` int32 [tokens];
-    ``partial_rows`` rows of partial results.  The arrays are numpy's until ``to`` moves them."""
+    """The work lists of a step's requests: ``items`` by kernel, int32 [n, 8] (``shared_prefix::Item``;
+    ``shapes``: their most rows and the unit of their ranges), ``seqs`` int32 [requests, 8]
+    (``shared_prefix::Joined``), ``token_seq`` int32 [tokens]; ``partial_rows`` rows of partial results, at
+    most ``most_parts`` of one row; ``turns``: some items leave two.  The arrays are numpy's until ``to``
+    moves them."""
     items: dict
     shapes: dict
     seqs: "np.ndarray | torch.Tensor"
     token_seq: "np.ndarray | torch.Tensor"
     partial_rows: int
-    most_parts: int          # partial results of a row, at most
+    most_parts: int
     tokens: int
     device: "torch.device | None" = field(default=None)
+    turns: bool = False
 
     def to(self, device: "torch.device | str") -> "SharedPlan":
         move = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(device)
         seqs = move(self.seqs)
         return SharedPlan({name: move(a) for name, a in self.items.items()}, self.shapes, seqs,
-                          move(self.token_seq), self.partial_rows, self.most_parts, self.tokens, seqs.device)
+                          move(self.token_seq), self.partial_rows, self.most_parts, self.tokens, seqs.device,
+                          self.turns)
 
 
 @dataclass(frozen=True)
@@ -58,12 +62,13 @@ class Tile:
     blocks: int
     places: int = 1
     least: int = 1
+    overhead: int = 256
 
 
 def choose_range(lengths: np.ndarray, copies: np.ndarray, tile: Tile) -> int:
     """How long the ranges are that ``lengths`` are cut into, a multiple of the tile's unit: each range of
     length i is the work of ``copies[i]`` blocks.  Of all numbers of rounds of as many blocks as the device
-    holds the one that is done first, a block costing its keys and as much as ``OVERHEAD`` keys besides."""
+    holds the one that is done first, a block costing its keys and the tile's ``overhead``."""
     longest, unit, blocks = int(lengths.max(initial=0)), tile.unit, tile.blocks
     whole = -(-longest // unit) * unit
     best = None
@@ -78,13 +83,10 @@ def choose_range(lengths: np.ndarray, copies: np.ndarray, tile: Tile) -> int:
                 high = mid
             else:
                 low = mid + 1
-        cost = rounds * (low * unit + OVERHEAD)
+        cost = rounds * (low * unit + tile.overhead)
         if best is None or cost < best[0]:
             best = (cost, low * unit)
     return best[1]
-
-
-OVERHEAD = 256
 
 
 
@@ -180,7 +182,8 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
     names = sorted(items, key=lambda name: (name != "tcgen05", name))
     return SharedPlan({name: np.concatenate(items[name]) for name in names}, shapes, seqs,
                       np.repeat(np.arange(len(qlen)), qlen), base,
-                      int((seqs[:, 3] + seqs[:, 6]).max(initial=0)), total)
+                      int((seqs[:, 3] + seqs[:, 6]).max(initial=0)), total,
+                      turns=any(t.places > 1 for members in by_name.values() for _, t in members))
 
 
 class SharedPrefixAttention:
@@ -236,8 +239,8 @@ class SharedPrefixAttention:
             # 55.5 and 39.7; 20 rows behind 2,040 of 8 17.9 and 18.7; 37 rows behind 6,373 of 32 40.6 and,
             # three tiles, 44.2; 48 rows behind 1,214 of 4, head size 64, 16.0 and 12.5)
             if rows > 32 and wide:
-                return (Tile("tcgen05", 128, 128, sms, 2, least=256) if rows <= 128 else
-                        Tile("tcgen05", 256, 128, sms))
+                return (Tile("tcgen05", 128, 128, sms, 2, least=256, overhead=512) if rows <= 128 else
+                        Tile("tcgen05", 256, 128, sms, overhead=512))
             return few
 
         return shared, lambda rows, keys: few
@@ -317,7 +320,8 @@ class SharedPrefixAttention:
             work = (*before, items.data_ptr(), items.shape[0])
             if (name == "tcgen05" and wide and not i
                     and (kernel := library.load(*self.tcgen05_module)).de_shared_tcgen05_page_ok(page)):
-                _check(kernel.de_shared_tcgen05(*work, *after), "shared prefix attention (tcgen05)")
+                _check(kernel.de_shared_tcgen05(*work, plan.turns, *after),
+                       "shared prefix attention (tcgen05)")
             elif name.startswith("f32") and pages_fit:
                 _check(library.load("shared_prefix_f32").de_shared_f32(*work, rows, order, *after),
                        "shared prefix attention (float32)")
