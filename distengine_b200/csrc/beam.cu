@@ -94,16 +94,24 @@ __device__ __forceinline__ float exponent_of(float top) {
 
 // A threshold with which `count(t)`, the number of keys of at least t over the block, lies between
 // `want` and `most`, or all keys but 0 where there are at most `most`.  `low` is a guess from below
-// (1: none), `top` the largest key; the range between is halved until it is met, which distinct keys
-// guarantee for most >= want (keys that are the same end with the largest threshold that has
-// `want`).  `count` is called by all threads.
-template <typename Count>
-__device__ __forceinline__ u64 threshold(u64 low, u64 top, int want, int most, Count count) {
+// (1: none), `lower()` another where the first leaves too few, `top` the largest key; the range between is
+// halved until it is met, which distinct keys guarantee for most >= want (keys that are the same end
+// with the largest threshold that has `want`).  `count` and `lower` are called by all threads.
+template <typename Count, typename Lower>
+__device__ __forceinline__ u64 threshold(u64 low, Lower lower, u64 top, int want, int most, Count count) {
     u64 high = top;
     if (low > 1) {
-        const int n = count(low);
+        int n = count(low);
         if (n >= want && n <= most) return low;
-        if (n < want) { high = low - 1; low = 1; }
+        if (n < want) {
+            high = low - 1;
+            low = lower();
+            if (low > 1) {
+                n = count(low);
+                if (n >= want && n <= most) return low;
+                if (n < want) { high = low - 1; low = 1; }
+            }
+        }
     }
     if (low <= 1) {
         if (top == 0 || count(1) <= most) return 1;
@@ -270,19 +278,30 @@ beam_slices_kernel(const float* __restrict__ logits, long long stride, int vocab
         sum += (double)terms(v);
     }
     __syncthreads();
-    // The largest; and a guess at the last of the `take` largest segments: as many parts of the block as
-    // are taken have each a segment of at least the smallest part's largest.
+    // The largest; and a guess at the last of the `take` largest segments: where as many parts of the block as
+    // are taken hold a number, each has a segment of at least the smallest part's largest.
+    // (Part p has every 64th segment from p on, so that few segments are spread over all parts.)
     unsigned mine = 0;
-    for (int i = tid; i < segments; i += SLICE_THREADS) mine = max(mine, segment_s[i]);
+    for (int i = (tid & 7) * (SLICE_THREADS / 8) + (tid >> 3); i < segments; i += SLICE_THREADS)
+        mine = max(mine, segment_s[i]);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
     if ((lane & 7) == 0) part_top[tid >> 3] = mine;
     __syncthreads();
     const unsigned x = part_top[2 * lane], y = part_top[2 * lane + 1];
-    unsigned guess = take > 32 ? min(x, y) : max(x, y);
-    if (take <= 16) guess = max(guess, __shfl_xor_sync(0xffffffffu, guess, 1));
-    guess = __reduce_min_sync(0xffffffffu, guess);
     const unsigned top = __reduce_max_sync(0xffffffffu, max(x, y));
+    unsigned guess = max(x, y);
+    if (take <= 16) guess = max(guess, __shfl_xor_sync(0xffffffffu, guess, 1));
+    int parts = __popc(__ballot_sync(0xffffffffu, guess > NOTHING));
+    if (take <= 16) parts >>= 1;
+    guess = guess > NOTHING ? guess : 0xffffffffu;
+    if (take > 32) {                                      // each of the two for itself
+        parts = __popc(__ballot_sync(0xffffffffu, x > NOTHING)) +
+                __popc(__ballot_sync(0xffffffffu, y > NOTHING));
+        guess = min(x > NOTHING ? x : 0xffffffffu, y > NOTHING ? y : 0xffffffffu);
+    }
+    guess = __reduce_min_sync(0xffffffffu, guess);
+    if (parts < take) guess = 0;
     const float m = top > NOTHING ? key_logit((u64)top << 32) : -INFINITY;
 
     sum = shfl_sum(sum * power_of_two(r - exponent_of(m)));
@@ -306,8 +325,9 @@ beam_slices_kernel(const float* __restrict__ logits, long long stride, int vocab
         if (tid == 0) counts_s[turn == 2 ? 0 : turn + 1] = 0;
         return k;
     };
-    const u64 last = threshold(guess > NOTHING ? (u64)guess << 32 : 1, (u64)top << 32 | 0xffffffffu, take,
-                               min(max(6 * take, 96), WINNERS), segments_from);
+    const u64 last = threshold(guess > NOTHING ? (u64)guess << 32 : 1, [] { return (u64)1; },
+                               (u64)top << 32 | 0xffffffffu, take, min(max(6 * take, 96), WINNERS),
+                               segments_from);
     if (tid == 0) winners_s = 0;
     __syncthreads();
     for (int i = tid; i < segments; i += SLICE_THREADS)
@@ -478,6 +498,7 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
     unsigned formed = 0;                                  // rows whose sums are 64-bit ones
     int found;
     for (;;) {
+        if (tid == 0) count_s = 0;
         __syncthreads();
         const unsigned again = again_s & ~formed;
         formed |= again;
@@ -502,48 +523,72 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
             }
             __syncthreads();
         }
-        // the largest, and a guess at the last one wanted: the largest last one of a slice
-        u64 top = 0, guess = 0;
-        for (int c = tid; c < n; c += JOIN_THREADS) {
-            const u64 t = key_s[c] ? total_key(total_of(c)) : 0;
-            total_s[c] = t;
-            top = max(top, t);
-        }
-        for (int i = tid; i < beams * slices; i += JOIN_THREADS) {
-            const int c = i * take + take - 1;
-            if (key_s[c]) guess = max(guess, total_key(total_of(c)));
-        }
-        top = warp_largest(top);
-        guess = warp_largest(guess);
-        if (lane == 0) { warp_part[0][warp] = top; warp_part[1][warp] = guess; }
-        if (tid == 0) count_s = 0;
-        __syncthreads();
-        for (int w = 0; w < JOIN_THREADS / 32; ++w) {
-            top = max(top, warp_part[0][w]);
-            guess = max(guess, warp_part[1][w]);
-        }
-
-        // the best by their totals; of those with the total of the last place the first by `place`
-        const u64 t0 = threshold(guess, top, want, most, [&](u64 t) {
-            return over_block([&](int c) { return total_s[c] >= t; });
-        });
-        u64 last = ~0ull;
-        if (over_block([&](int c) { return total_s[c] >= t0; }) > most) {
-            const int above = over_block([&](int c) { return total_s[c] > t0; });
-            u64 low = 0, high = ~0ull;
-            while (low < high) {
-                const u64 mid = low + ((high - low) >> 1);
-                const int k = over_block([&](int c) { return total_s[c] == t0 && place(c) <= mid; });
-                if (above + k >= want) high = mid; else low = mid + 1;
+        if (n <= PICKS / 2) {                             // few: all are ranked
+            for (int c = tid; c < n; c += JOIN_THREADS) {
+                const u64 t = key_s[c] ? total_key(total_of(c)) : 0;
+                total_s[c] = t;
+                if (t) {
+                    const int at = atomicAdd(&count_s, 1);
+                    pick_s[at] = c;
+                    pick_total_s[at] = t;
+                }
             }
-            last = high;
-        }
-        for (int c = tid; c < n; c += JOIN_THREADS) {
-            const u64 t = total_s[c];
-            if (t > t0 || (t == t0 && t != 0 && place(c) <= last)) {
-                const int at = atomicAdd(&count_s, 1);
-                pick_s[at] = c;
-                pick_total_s[at] = t;
+        } else {
+            // the largest, and a guess at the last one wanted: the largest last one of a slice, of which
+            // there is one more than are wanted unless they are all in that slice; then the next largest
+            u64 top = 0, guess = 0;
+            for (int c = tid; c < n; c += JOIN_THREADS) {
+                const u64 t = key_s[c] ? total_key(total_of(c)) : 0;
+                total_s[c] = t;
+                top = max(top, t);
+            }
+            for (int i = tid; i < beams * slices; i += JOIN_THREADS) {
+                const int c = i * take + take - 1;
+                if (key_s[c]) guess = max(guess, total_key(total_of(c)));
+            }
+            top = warp_largest(top);
+            guess = warp_largest(guess);
+            if (lane == 0) { warp_part[0][warp] = top; warp_part[1][warp] = guess; }
+            __syncthreads();
+            for (int w = 0; w < JOIN_THREADS / 32; ++w) {
+                top = max(top, warp_part[0][w]);
+                guess = max(guess, warp_part[1][w]);
+            }
+
+            // the best by their totals; of those with the total of the last place the first by `place`
+            auto next = [&] {
+                u64 v = 0;
+                for (int i = tid; i < beams * slices; i += JOIN_THREADS) {
+                    const int c = i * take + take - 1;
+                    if (key_s[c] && total_s[c] < guess) v = max(v, total_s[c]);
+                }
+                v = warp_largest(v);
+                if (lane == 0) warp_part[0][warp] = v;
+                __syncthreads();
+                for (int w = 0; w < JOIN_THREADS / 32; ++w) v = max(v, warp_part[0][w]);
+                return max(v, (u64)1);
+            };
+            const u64 t0 = threshold(guess, next, top, want, most, [&](u64 t) {
+                return over_block([&](int c) { return total_s[c] >= t; });
+            });
+            u64 last = ~0ull;
+            if (over_block([&](int c) { return total_s[c] >= t0; }) > most) {
+                const int above = over_block([&](int c) { return total_s[c] > t0; });
+                u64 low = 0, high = ~0ull;
+                while (low < high) {
+                    const u64 mid = low + ((high - low) >> 1);
+                    const int k = over_block([&](int c) { return total_s[c] == t0 && place(c) <= mid; });
+                    if (above + k >= want) high = mid; else low = mid + 1;
+                }
+                last = high;
+            }
+            for (int c = tid; c < n; c += JOIN_THREADS) {
+                const u64 t = total_s[c];
+                if (t > t0 || (t == t0 && t != 0 && place(c) <= last)) {
+                    const int at = atomicAdd(&count_s, 1);
+                    pick_s[at] = c;
+                    pick_total_s[at] = t;
+                }
             }
         }
         __syncthreads();
@@ -576,15 +621,20 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
     }
 }
 
-// Slices that a row is cut into, and their logits: as many blocks as the SMs hold at once (four each),
-// of no fewer than 2,048 logits.  (512 rows of 128,256 in one slice each, 512 blocks; in four, whose
-// ends of a few microseconds are then paid four times, 73 us instead of 61.)
+// Slices that a row is cut into, and their logits.  A block an SM; more, up to the four that an SM holds at
+// once, only of 32,768 logits and longer, since a block's end takes some microseconds (us with one and with up
+// to four blocks an SM: 64 rows of 32,000 10.7 and 16.8, 35 of 50,021 13.8 and 16.4, 186 of 79,707 28.7 and
+// 25.4).  No slice is shorter than 2,048 logits, and the slices of a group leave no more than 1,024 candidates,
+// for the block that joins them (eight rows of 128,256, 16 taken, with 512, 1,024, 2,048 and 8,192: 16.2, 14.0,
+// 14.2 and 23.9).
 struct Slicing {
     int slices, elements;
 };
-constexpr int JOIN_MOST = 8192;                           // candidates of a group in shared memory
+constexpr int JOIN_MOST = 1024;
 Slicing slicing(int rows, int beams, int vocab, int take) {
-    int slices = rows > 0 ? 4 * 148 / rows : 1;
+    int slices = rows > 0 ? 148 / rows : 1;
+    const int longer = rows > 0 ? 4 * 148 / rows : 1, whole = vocab / 32768;
+    if (slices < longer && slices < whole) slices = longer < whole ? longer : whole;
     const int least = vocab / (4 * SLICE_THREADS), most = JOIN_MOST / (beams * take);
     if (slices > least) slices = least;
     if (slices > most) slices = most;
@@ -728,12 +778,7 @@ DE_EXPORT int de_beam_select(const float* logits, long long stride, const float*
     float* maxima = (float*)scratch;
     double* sums = (double*)((char*)scratch + aligned(4 * n));
     u64* keys = (u64*)((char*)sums + aligned(8 * n));
-    const int totals = 2 * beams * s.slices * take * 8;
-    if (totals > 32 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(
-            beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, totals);
-        if (e != cudaSuccess) return (int)e;
-    }
+    const int totals = 2 * beams * s.slices * take * 8;   // (up to 32 KB)
     const int code = de_launch(beam_slices_kernel, dim3((unsigned)n), dim3(SLICE_THREADS), 0,
                                (cudaStream_t)stream, logits, stride, vocab, s.elements, s.slices, take,
                                maxima, sums, keys);

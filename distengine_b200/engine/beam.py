@@ -150,6 +150,7 @@ class BeamSearch:
                                                      [len(portion) - 1] if last else [])])
             search.tokens, search.scores = [[]] * self.beams, [0.0] + [NO_SCORE] * (self.beams - 1)
             candidates = self.selector.select(logits, [[0.0]], self.take)[0]
+            self.runner.check_status()
             _, tokens = choose(search, candidates, self.beams, eos, self.penalty)
             if max_new_tokens > 1 and not is_done(search, self.beams, self.penalty):
                 self.cache.fork(search.ids[0], search.ids[1:])
