@@ -270,9 +270,9 @@ shared_merge_kernel(T* __restrict__ out, int out_stride, const int* __restrict__
 }
 
 // A warp alone reads up to MERGE_FEW results a row, four at once or eight; more are shared out over four
-// warps.  (us for all launches: 18 questions of 21 tokens behind two documents of 4,100 keys, where a row has
-// some ten results, 42.9 with a warp and 38.2 with four; 16 requests behind 4,096 keys, 32 heads of 64, 65
-// results, 25.2 and 14.4; 64 requests behind 16 prompts of 1,003 keys, five results, 55.5 and 57.5.)
+// warps.  (us for all launches, a warp and four: 16 requests behind 4,096 keys, 32 heads of 64, 65 results a
+// row, 25.2 and 14.4; four beams behind 512 keys, nine results, 7.5 and 7.2; 64 requests behind 16 prompts of
+// 1,003 keys, five results, 55.5 and 57.5.)
 template <typename T, int WARPS>
 int merge_with(void* out, int out_stride, const int* token_seq, const int* seqs, const float* partial_acc,
                const float* partial_ml, int tokens, int heads, int kv_heads, int d, cudaStream_t stream) {

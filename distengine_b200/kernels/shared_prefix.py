@@ -13,7 +13,7 @@ nothing between requests.
 
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 
 import numpy as np
 import torch
@@ -55,7 +55,11 @@ class Tile:
     """A tile of a kernel: the kernel's name among the plan's items, query rows, keys that a range is a
     multiple of (one number for all tiles of a kernel), blocks (or warps, where those have an item
     each) that the device holds at once; ``places``: partial results that a range leaves; ``least``: keys
-    of the shortest range that is worth a block."""
+    of the shortest range that is worth a block; ``overhead``: keys that take as long as a block's beginning
+    and end (tcgen05: 108 rows behind 15,566 keys of 32 kv heads 86 us with 512, 92 with 256); ``own_key``:
+    a block has an SM to itself, and this is what a request's own key for 16 rows takes of an SM in keys of
+    this tile (64 requests behind 8,192 keys with 500 of their own 45 us with 64 blocks and the own keys'
+    beside them, 50 with 128 and those behind them; 43 + 43 behind 463 with 242 21 and 28)."""
     name: str
     rows: int
     unit: int
@@ -63,31 +67,47 @@ class Tile:
     places: int = 1
     least: int = 1
     overhead: int = 256
+    own_key: float = 0.0
 
 
-def choose_range(lengths: np.ndarray, copies: np.ndarray, tile: Tile) -> int:
-    """How long the ranges are that ``lengths`` are cut into, a multiple of the tile's unit: each range of
-    length i is the work of ``copies[i]`` blocks.  Of all numbers of rounds of as many blocks as the device
-    holds the one that is done first, a block costing its keys and the tile's ``overhead``."""
+def choose_range(lengths: np.ndarray, copies: np.ndarray, tile: Tile,
+                 beside: float = 0.0) -> "tuple[int, float]":
+    """How long the ranges are that ``lengths`` are cut into, a multiple of the tile's unit, and how much of
+    the device they leave to others meanwhile: each range of length i is the work of ``copies[i]`` blocks.
+    Of all numbers of rounds of as many blocks as the device holds the one that is done first, a block
+    costing its keys and the tile's ``overhead``.  ``beside``: work of another kernel, in keys, whose blocks
+    find no room beside these: either it follows, or there are so few of these that both are done at
+    about the same time."""
     longest, unit, blocks = int(lengths.max(initial=0)), tile.unit, tile.blocks
     whole = -(-longest // unit) * unit
-    best = None
     fewest = max(1, -(-longest // (MAX_SPLITS * unit)), -(-min(tile.least, whole) // unit))
     count = lambda each: int((-(-lengths // each) * copies).sum())
-    least = -(-count(max(whole, unit)) // blocks)
-    for rounds in range(max(least, 1), max(least, 1) + 4):
-        low, high = fewest, max(whole // unit, fewest)    # the shortest that needs no more rounds
+
+    def shortest(most: int) -> int:                       # of which there are no more
+        low, high = fewest, max(whole // unit, fewest)
         while low < high:
             mid = (low + high) // 2
-            if count(mid * unit) <= rounds * blocks:
+            if count(mid * unit) <= most:
                 high = mid
             else:
                 low = mid + 1
-        cost = rounds * (low * unit + tile.overhead)
-        if best is None or cost < best[0]:
-            best = (cost, low * unit)
-    return best[1]
+        return low * unit
 
+    best = None
+    least = max(-(-count(max(whole, unit)) // blocks), 1)
+    for rounds in range(least, least + 4):
+        each = shortest(rounds * blocks)
+        cost = rounds * (each + tile.overhead) + beside / blocks
+        if best is None or cost < best[0]:
+            best = (cost, each, 0.0)
+    if beside > 0:
+        for eighths in range(6, 0, -1):
+            each = shortest(blocks * eighths // 8)
+            n = count(each)
+            cost = max(each + tile.overhead, beside / max(blocks - n, 1))
+            if n <= blocks * 3 // 4 and cost < best[0]:
+                best = (cost, each, 1 - n / blocks)
+    return best[1:]
 
 
 def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, prefix_tile,
@@ -123,15 +143,22 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
         items.setdefault(t.name, []).append(part)
         shapes[t.name] = (max(t.rows, shapes.get(t.name, (0, 0))[0]), t.unit)
 
+    # each request's own keys, behind its prefix
+    start = np.repeat(prefix, sizes)
+    own = np.maximum(int(tail), qlen) + np.where(start > 0, 0, np.repeat(shared, sizes))
+    own_keys = kv_heads * float((own * -(-qlen * group // 16)).sum())
+
     # shared keys
     by_name: dict[str, list] = {}
+    left = 0.0                                            # of the device, beside blocks that have SMs to themselves
     for g in np.nonzero((prefix > 0) & (rows > 0))[0]:
         t = prefix_tile(int(rows[g]), int(prefix[g]))
         by_name.setdefault(t.name, []).append((int(g), t))
     for members in by_name.values():
         lengths = prefix[[g for g, _ in members]]
         copies = np.asarray([-(-int(rows[g]) // t.rows) * kv_heads for g, t in members])
-        each = choose_range(lengths, copies, members[0][1])
+        each, beside = choose_range(lengths, copies, members[0][1], members[0][1].own_key * own_keys)
+        left = max(left, beside)
         for g, t in members:
             p, n = int(prefix[g]), int(rows[g])
             chunks, count = -(-p // each), -(-n // t.rows)
@@ -151,9 +178,7 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
             seqs[s, 2], seqs[s, 3], seqs[s, 4] = base, chunks * t.places, t.rows
             base += count * chunks * t.rows * t.places
 
-    # each request's own keys, behind its prefix
-    start = np.repeat(prefix, sizes)
-    own = np.maximum(int(tail), qlen) + np.where(start > 0, 0, np.repeat(shared, sizes))
+    # own keys
     by_tile: dict[Tile, list] = {}
     for s in np.nonzero(qlen > 0)[0]:
         by_tile.setdefault(own_tile(int(qlen[s]) * group, int(own[s])), []).append(int(s))
@@ -161,7 +186,9 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
         s = np.asarray(members)
         n = qlen[s] * group
         count = -(-n // t.rows)
-        each = choose_range(own[s], count * kv_heads, t)
+        if left:
+            t = replace(t, blocks=int(t.blocks * left))
+        each, _ = choose_range(own[s], count * kv_heads, t)
         splits = np.clip(-(-own[s] // each), 1, MAX_SPLITS)
         pieces = count * splits
         owner = np.repeat(np.arange(len(s)), pieces)
@@ -239,8 +266,8 @@ class SharedPrefixAttention:
             # 55.5 and 39.7; 20 rows behind 2,040 of 8 17.9 and 18.7; 37 rows behind 6,373 of 32 40.6 and,
             # three tiles, 44.2; 48 rows behind 1,214 of 4, head size 64, 16.0 and 12.5)
             if rows > 32 and wide:
-                return (Tile("tcgen05", 128, 128, sms, 2, least=256, overhead=512) if rows <= 128 else
-                        Tile("tcgen05", 256, 128, sms, overhead=512))
+                return (Tile("tcgen05", 128, 128, sms, 2, least=256, overhead=512, own_key=self.head_dim / 256) if rows <= 128 else
+                        Tile("tcgen05", 256, 128, sms, overhead=512, own_key=self.head_dim / 256))
             return few
 
         return shared, lambda rows, keys: few
