@@ -146,6 +146,8 @@ def _generate_from_folder(args: argparse.Namespace) -> int:
                                                           None) is not None else -1
     if args.beams > 1:
         found = engine.beam_search(prompts, args.max_new_tokens, args.beams, eos, args.length_penalty)
+        if not all(found):
+            raise SystemExit("a prompt has no continuation (its logits are not finite)")
         outputs = [hypotheses[0].token_ids for hypotheses in found]
     else:
         found = None

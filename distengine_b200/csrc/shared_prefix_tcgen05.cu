@@ -56,11 +56,10 @@ template <bool TURNS> __host__ __device__ constexpr int copy_warps() { return TU
 template <bool TURNS> __host__ __device__ constexpr int threads() { return (COPY_WARP + copy_warps<TURNS>()) * 32; }
 constexpr int SMEM = 2 * BUFFER + BUFFERS * BUFFER + 512 + 2 * 2 * LANES * 4;
 constexpr int COLUMNS = 512;
-// columns of tensor memory: scores of pipeline x at 128 x; results at 256 + D x; weights (64 columns) over
-// the scores at head size 128, where there is no other room, and at 384 + 64 x at head size 64
-constexpr bool OVER = D == 128;
+// columns of tensor memory: scores of pipeline x and half h of a tile at 128 x + 64 h, weights over the first
+// 32 of them; results at 256 + D x
 constexpr int O_COL = 256;
-__device__ __forceinline__ unsigned p_col(int x) { return OVER ? 128u * x : 384u + 64u * x; }
+constexpr int HK = KT / 2;                    // keys of a half
 constexpr float RAISE = 8.0f;
 constexpr int ROW_BYTES = D * 4 + 16;         // of a row's results in shared memory: no two lanes on one bank
 static_assert(2 * LANES * ROW_BYTES <= BUFFERS * BUFFER, "the ring holds the results");
@@ -216,7 +215,7 @@ __device__ __forceinline__ unsigned long long value_desc(const void* tile) {
     if (KS == 2) d += (unsigned long long)((SUB >> 4) - 1) << 16;
     return d;
 }
-constexpr unsigned DESC_S = instr_desc(128, KT);
+constexpr unsigned DESC_S = instr_desc(128, HK);
 constexpr unsigned DESC_O = instr_desc(128, D) | 1u << 16;
 
 template <bool B> struct Truth {
@@ -239,14 +238,13 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
     unsigned long long* bars = reinterpret_cast<unsigned long long*>(ring + BUFFERS * BUFFER);
     unsigned long long* full = bars;                      // [BUFFERS] the pages have landed
     unsigned long long* empty = bars + BUFFERS;           // [BUFFERS] the products that read it are done
-    unsigned long long* s_done = bars + 2 * BUFFERS;      // [2] scores are complete
-    unsigned long long* p_ready = s_done + 2;             // [2] weights are written (256 arrivals)
-    unsigned long long* o_done = s_done + 4;              // [2] weights times values is complete
-    unsigned long long* s_free = s_done + 6;              // [2] scores are in registers (256 arrivals)
-    unsigned long long* drained = s_done + 8;             // [2] what is issued is complete
-    unsigned long long* p_half = s_done + 10;             // [2] those of the first 64 keys are
-    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(s_done + 12);
-    int& missing_s = *reinterpret_cast<int*>(s_done + 13);
+    // of each pipeline and half of a tile:
+    unsigned long long* s_done = bars + 2 * BUFFERS;      // [2][2] scores are complete
+    unsigned long long* p_ready = s_done + 4;             // [2][2] weights are written (256 arrivals)
+    unsigned long long* o_done = s_done + 8;              // [2][2] weights times values is complete
+    unsigned long long* drained = s_done + 12;            // [2] what is issued is complete
+    unsigned& tmem_slot = *reinterpret_cast<unsigned*>(s_done + 14);
+    int& missing_s = *reinterpret_cast<int*>(s_done + 15);
     int* issued_s = &missing_s + 1;                       // units whose copies have begun
     float* exchange = reinterpret_cast<float*>(ring + BUFFERS * BUFFER + 512);   // [pipeline][half][row]
 
@@ -272,12 +270,10 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             mbar_init(&full[i], COPIERS);
             mbar_init(&empty[i], !turns && it.count > LANES ? 2 : 1);      // pipelines that read it
         }
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < 4; ++x) {
             mbar_init(&s_done[x], 1);
             mbar_init(&p_ready[x], 2 * LANES);
-            mbar_init(&p_half[x], 2 * LANES);
             mbar_init(&o_done[x], 1);
-            mbar_init(&s_free[x], 2 * LANES);
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -384,41 +380,48 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             after_sync();
             return ok;
         };
-        // (a buffer's wait first: it is over long before the other one nearly always)
-        auto scores = [&](int j, void* bar, unsigned parity) {
-            const int unit = 2 * tile_of(i, j), b = unit % BUFFERS;
-            landed(unit);
-            if (!passed(bar, parity)) return;
+        // step u is half u % 2 of the pipeline's tile u / 2; use u / 2 of the half's barriers
+        auto scores = [&](int u) {
+            const int h = u & 1, unit = 2 * tile_of(i, u >> 1), b = unit % BUFFERS;
+            if (h == 0) landed(unit);
+            // (the half's columns hold the weights of two steps before)
+            if (u >= 2 && !passed(&o_done[2 * i + h], ((u >> 1) - 1) & 1)) return;
+            if (u < 2) {
+                ok = __all_sync(0xffffffffu, ok);
+                after_sync();
+            }
+            if (!ok) return;
 #pragma unroll
             for (int sub = 0; sub < KS; ++sub) {
                 const unsigned long long a = smem_desc(q_s + i * BUFFER + sub * SUB);
-                const unsigned long long kb = smem_desc(ring + b * BUFFER + sub * SUB);
+                const unsigned long long kb = smem_desc(ring + b * BUFFER + sub * SUB + h * (SUB / 2));
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    umma(tmem + 128 * i, a + 2 * k, kb + 2 * k, DESC_S, sub > 0 || k > 0);
+                    umma(tmem + 128 * i + HK * h, a + 2 * k, kb + 2 * k, DESC_S, sub > 0 || k > 0);
             }
-            commit(&s_done[i]);
-            commit(&empty[b]);
+            commit(&s_done[2 * i + h]);
+            if (h == 1) commit(&empty[b]);
         };
-        if (n > 0) scores(0, &full[2 * tile_of(i, 0)], 0);
-        for (int j = 0; j < n && ok; ++j) {
-            if (!OVER && j + 1 < n) scores(j + 1, &s_free[i], j & 1);     // once these are in registers
-            const int unit = 2 * tile_of(i, j) + 1, b = unit % BUFFERS;
+        if (n > 0) scores(0);
+        for (int u = 0; u < 2 * n && ok; ++u) {
+            const int h = u & 1;
+            // the next scores while this step's exponentials are formed; but where the pipelines take turns
+            // the next tile's keys may be far, and this tile's values are released first
+            const bool early = !turns || h == 0;
+            if (early && u + 1 < 2 * n) scores(u + 1);
+            if (!ok) break;
+            const int unit = 2 * tile_of(i, u >> 1) + 1, b = unit % BUFFERS;
             const unsigned long long vb = value_desc(ring + b * BUFFER);
-            landed(unit);
-            if (!passed(&p_half[i], j & 1)) break;
+            if (h == 0) landed(unit);
+            if (!passed(&p_ready[2 * i + h], (u >> 1) & 1)) break;
 #pragma unroll
-            for (int k = 0; k < KT / 32; ++k)
-                umma_a_tmem(tmem + O_COL + D * i, tmem + p_col(i) + 8 * k,
-                            vb + (unsigned long long)(k * 2048 >> 4), DESC_O, j > 0 || k > 0);
-            if (!passed(&p_ready[i], j & 1)) break;
-#pragma unroll
-            for (int k = KT / 32; k < KT / 16; ++k)
-                umma_a_tmem(tmem + O_COL + D * i, tmem + p_col(i) + 8 * k,
-                            vb + (unsigned long long)(k * 2048 >> 4), DESC_O, true);
-            commit(&o_done[i]);
-            commit(&empty[b]);
-            if (OVER && j + 1 < n) scores(j + 1, &o_done[i], j & 1);      // the weights lie where they will
+            for (int k = 0; k < HK / 16; ++k)
+                umma_a_tmem(tmem + O_COL + D * i, tmem + 128 * i + HK * h + 8 * k,
+                            vb + (unsigned long long)((h * (HK / 16) + k) * 2048 >> 4), DESC_O,
+                            u > 0 || k > 0);
+            commit(&o_done[2 * i + h]);
+            if (h == 1) commit(&empty[b]);
+            if (!early && u + 1 < 2 * n) scores(u + 1);
         }
         // what is issued, the last buffers' commits with it, ends before the block does
         commit(&drained[i]);
@@ -428,66 +431,53 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         // ------------------------------------------------------------------ softmax
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
         const unsigned s_addr = tmem + 128 * x + 32 * half + lanes;
-        const unsigned p_addr = tmem + p_col(x) + 16 * half + lanes;
+        const unsigned p_addr = tmem + 128 * x + 16 * half + lanes;
         const unsigned o_addr = tmem + O_COL + D * x + D / 2 * half + lanes;
         const int pair = 1 + 4 * x + (warp & 3);          // the barrier of the two warps of the same rows
         float* mine = exchange + (2 * x + half) * LANES + rowi;
         float* other = exchange + (2 * x + (half ^ 1)) * LANES + rowi;
         const float sl = scale * 1.4426950408889634f;
         float m_ref = -INFINITY, l_run = 0.0f;
-        // EDGE: a tile in which keys are hidden (a form of its own, so that the others' code is free of it)
-        auto tile = [&](int j, auto edge) {
+        // step u, as above; EDGE: keys are hidden (a form of its own, so that the others' code is free of it)
+        auto step = [&](int u, auto edge) {
             constexpr bool EDGE = decltype(edge)::value;
-            const int t = tile_of(x, j), kt = it.begin + t * KT;
-            if (ok) ok = wait(&s_done[x], j & 1, status);
+            const int h = u & 1, t = tile_of(x, u >> 1), kt = it.begin + t * KT;
+            if (ok) ok = wait(&s_done[2 * x + h], (u >> 1) & 1, status);
             __syncwarp();
             after_sync();
-            unsigned sv[2][32];
-            tmem_load_32cols(s_addr, sv[0]);
-            tmem_load_32cols(s_addr + 64, sv[1]);
+            unsigned sv[32];
+            tmem_load_32cols(s_addr + HK * h, sv);
             tmem_wait_loads();
-            if (!OVER) {
-                before_sync();
-                mbar_arrive(&s_free[x]);
-            }
             // keys behind the range, or without a page, are not seen
             unsigned gone = 0;                            // boxes without a page
             if constexpr (EDGE) {
                 const int key = kt + lane * box;
                 gone = __ballot_sync(0xffffffffu, lane < boxes && key < it.end && page_at(key) < 0);
+                const int n = HK * h + 32 * half + lane;
+                const unsigned seen =
+                    __ballot_sync(0xffffffffu, kt + n < it.end && !(gone >> (n / box) & 1));
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int n = 64 * c + 32 * half + lane;
-                    const unsigned seen =
-                        __ballot_sync(0xffffffffu, kt + n < it.end && !(gone >> (n / box) & 1));
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (!(seen >> i & 1)) sv[c][i] = 0xff800000u;
-                }
+                for (int i = 0; i < 32; ++i)
+                    if (!(seen >> i & 1)) sv[i] = 0xff800000u;
             }
             float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
+            for (int i = 0; i < 32; i += 8)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    m4[c] = max_three(m4[c], sv[c][i], sv[c][i + 1]);
-                    m4[c + 2] = max_three(m4[c + 2], sv[c][i + 2], sv[c][i + 3]);
-                }
+                for (int c = 0; c < 4; ++c) m4[c] = max_three(m4[c], sv[i + 2 * c], sv[i + 2 * c + 1]);
             const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            bool rest = OVER || j == 0;                   // the last product is known to be complete
             if (any_of_pair(pair, (m - m_ref) * sl > RAISE)) {
-                if (!rest) {
-                    if (ok) ok = wait(&o_done[x], (j - 1) & 1, status);
+                if (u > 0) {                              // no product adds to the results meanwhile
+                    if (ok) ok = wait(&o_done[2 * x + (h ^ 1)], ((u - 1) >> 1) & 1, status);
                     __syncwarp();
                     after_sync();
-                    rest = true;
                 }
                 *mine = m;
                 sync_pair(pair);
                 const float top = fmaxf(m, *other);       // of the row
                 const bool raise = (top - m_ref) * sl > RAISE;
                 const float f = raise ? exp2_fast((m_ref - top) * sl) : 1.0f;
-                if (j > 0) {
+                if (u > 0) {
 #pragma unroll 1
                     for (int c = 0; c < D / 32; ++c) {
                         unsigned ov[16];
@@ -507,61 +497,51 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             }
             const float off = m_ref == -INFINITY ? 0.0f : -m_ref * sl;
             const Two sl2 = two(sl, sl), off2 = two(off, off);
-            if (!rest) {                                  // the weights' columns are free
-                if (ok) ok = wait(&o_done[x], (j - 1) & 1, status);
-                __syncwarp();
-                after_sync();
-            }
             Two sum2[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
+            unsigned pw[16];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                unsigned pw[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float a, b;
-                    untwo(fma_two(two(__uint_as_float(sv[c][2 * i]), __uint_as_float(sv[c][2 * i + 1])),
-                                  sl2, off2), a, b);
-                    a = exp2_fast(a);
-                    b = exp2_fast(b);
-                    sum2[i & 1] = add_two(sum2[i & 1], two(a, b));
-                    pw[i] = pack2(a, b);
-                }
-                tmem_store_16cols(p_addr + 32 * c, pw);
-                if (c == 0) {
-                    // Values that no row sees may be anything, and 0 * NaN is NaN in the product: the
-                    // first thread of row i has the values of key i (both pipelines write the same zeros).
-                    if (EDGE && half == 0 && (kt + rowi >= it.end || (gone >> (rowi / box) & 1))) {
-                        const int unit = 2 * t + 1, b = unit % BUFFERS;
-                        landed(unit);
-#pragma unroll
-                        for (int sub = 0; sub < KS; ++sub) {
-                            uint4* v = reinterpret_cast<uint4*>(ring + b * BUFFER + sub * SUB + rowi * 128);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) v[e] = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                    }
-                    if constexpr (EDGE) __syncwarp();
-                    tmem_wait_stores();
-                    before_sync();
-                    mbar_arrive(&p_half[x]);
-                }
+            for (int i = 0; i < 16; ++i) {
+                float a, b;
+                untwo(fma_two(two(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sl2, off2),
+                      a, b);
+                a = exp2_fast(a);
+                b = exp2_fast(b);
+                sum2[i & 1] = add_two(sum2[i & 1], two(a, b));
+                pw[i] = pack2(a, b);
             }
+            tmem_store_16cols(p_addr + HK * h, pw);
             {
                 float a, b;
                 untwo(add_two(sum2[0], sum2[1]), a, b);
                 l_run += a + b;
             }
+            // Values that no row sees may be anything, and 0 * NaN is NaN in the product: the first thread of
+            // row i has the values of key i (both pipelines write the same zeros).
+            if constexpr (EDGE) {
+                if (half == 0 && rowi / HK == h &&
+                    (kt + rowi >= it.end || (gone >> (rowi / box) & 1))) {
+                    const int unit = 2 * t + 1, b = unit % BUFFERS;
+                    landed(unit);
+#pragma unroll
+                    for (int sub = 0; sub < KS; ++sub) {
+                        uint4* v = reinterpret_cast<uint4*>(ring + b * BUFFER + sub * SUB + rowi * 128);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                }
+                __syncwarp();
+            }
             tmem_wait_stores();
             before_sync();
-            mbar_arrive(&p_ready[x]);
+            mbar_arrive(&p_ready[2 * x + h]);
         };
-        for (int j = 0; j < n_of[x]; ++j) {
-            if (missing || it.begin + (tile_of(x, j) + 1) * KT > it.end) tile(j, Truth<true>());
-            else tile(j, Truth<false>());
+        for (int u = 0; u < 2 * n_of[x]; ++u) {
+            if (missing || it.begin + (tile_of(x, u >> 1) + 1) * KT > it.end) step(u, Truth<true>());
+            else step(u, Truth<false>());
         }
         if (n_of[x] > 0) {
-            if (ok) ok = wait(&o_done[x], (n_of[x] - 1) & 1, status);
+            if (ok) ok = wait(&o_done[2 * x + 1], (n_of[x] - 1) & 1, status);
             __syncwarp();
             after_sync();
         }

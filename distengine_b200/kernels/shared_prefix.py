@@ -31,7 +31,8 @@ class SharedPlan:
     ``shapes``: their most rows and the unit of their ranges), ``seqs`` int32 [requests, 8]
     (``shared_prefix::Joined``), ``token_seq`` int32 [tokens]; ``partial_rows`` rows of partial results, at
     most ``most_parts`` of one row; ``turns``: some items leave two.  The arrays are numpy's until ``to``
-    moves them."""
+    moves them.  (Kernels read them before the kernel in front of theirs has ended: on the device they come
+    from copies, as ``to`` and a step's upload make them.)"""
     items: dict
     shapes: dict
     seqs: "np.ndarray | torch.Tensor"
