@@ -200,7 +200,8 @@ class AttentionLauncher:
         prep.notes[self.key] = ()
         prep.notes[self.key + "/decode"] = None
         prep.notes[self.key + "/shared"] = (tuple(plan.shapes.items()), tuple(plan.items),
-                                            plan.partial_rows, plan.most_parts, plan.tokens)
+                                            plan.partial_rows, plan.most_parts, plan.tokens,
+                                            plan.turns)
         return True
 
     def _prepare_decode(self, prep, force_split: "tuple[int, int, int] | None") -> None:
@@ -378,11 +379,11 @@ class AttentionLauncher:
                    v_pages: torch.Tensor, block_table: torch.Tensor, ctx) -> None:
         """A step of single tokens whose requests share prefixes; arguments as ``run``."""
         from .shared_prefix import SharedPlan
-        shapes, names, partial_rows, most_parts, tokens = ctx.notes[self.key + "/shared"]
+        shapes, names, partial_rows, most_parts, tokens, turns = ctx.notes[self.key + "/shared"]
         at = f"{self.key}/shared/"
         plan = SharedPlan({name: ctx.arrays[at + name] for name in names}, dict(shapes),
                           ctx.arrays[at + "seqs"], ctx.arrays[at + "token_seq"], partial_rows, most_parts,
-                          tokens, q.device)
+                          tokens, q.device, turns)
         self.shared.run(q, out, k_pages, v_pages, block_table, ctx.seq_slot, ctx.seq_pos0, plan,
                         ctx.status, ctx.buffer)
 

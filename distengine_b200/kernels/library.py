@@ -173,7 +173,7 @@ SIGNATURES: dict[str, dict[str, list]] = {
     },
     "shared_prefix_tcgen05": {
         "de_shared_tcgen05_page_ok": [I],
-        "de_shared_tcgen05": [P, I, P, P, P, I, I, P, P, P, I, P, P, I, I, I, I, F, P, P],
+        "de_shared_tcgen05": [P, I, P, P, P, I, I, P, P, P, I, I, P, P, I, I, I, I, F, P, P],
     },
     "attention_decode": {
         "de_attn_decode_head_dim": [], "de_attn_decode_max_cluster": [],

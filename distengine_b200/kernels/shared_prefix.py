@@ -30,9 +30,9 @@ class SharedPlan:
     """The work lists of a step's requests: ``items`` by kernel, int32 [n, 8] (``shared_prefix::Item``;
     ``shapes``: their most rows and the unit of their ranges), ``seqs`` int32 [requests, 8]
     (``shared_prefix::Joined``), ``token_seq`` int32 [tokens]; ``partial_rows`` rows of partial results, at
-    most ``most_parts`` of one row.  The arrays are numpy's until ``to`` moves them.  (Kernels read them
-    before the kernel in front of theirs has ended: on the device they come from copies, as ``to`` and a
-    step's upload make them.)"""
+    most ``most_parts`` of one row; ``turns``: some items leave two.  The arrays are numpy's until ``to``
+    moves them.  (Kernels read them before the kernel in front of theirs has ended: on the device they come
+    from copies, as ``to`` and a step's upload make them.)"""
     items: dict
     shapes: dict
     seqs: "np.ndarray | torch.Tensor"
@@ -41,12 +41,14 @@ class SharedPlan:
     most_parts: int
     tokens: int
     device: "torch.device | None" = field(default=None)
+    turns: bool = False
 
     def to(self, device: "torch.device | str") -> "SharedPlan":
         move = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(device)
         seqs = move(self.seqs)
         return SharedPlan({name: move(a) for name, a in self.items.items()}, self.shapes, seqs,
-                          move(self.token_seq), self.partial_rows, self.most_parts, self.tokens, seqs.device)
+                          move(self.token_seq), self.partial_rows, self.most_parts, self.tokens, seqs.device,
+                          self.turns)
 
 
 @dataclass(frozen=True)
@@ -208,7 +210,8 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
     names = sorted(items, key=lambda name: (name != "tcgen05", name))
     return SharedPlan({name: np.concatenate(items[name]) for name in names}, shapes, seqs,
                       np.repeat(np.arange(len(qlen)), qlen), base,
-                      int((seqs[:, 3] + seqs[:, 6]).max(initial=0)), total)
+                      int((seqs[:, 3] + seqs[:, 6]).max(initial=0)), total,
+                      turns=any(t.places > 1 for members in by_name.values() for _, t in members))
 
 
 class SharedPrefixAttention:
@@ -345,7 +348,8 @@ class SharedPrefixAttention:
             work = (*before, items.data_ptr(), items.shape[0])
             if (name == "tcgen05" and wide and not i
                     and (kernel := library.load(*self.tcgen05_module)).de_shared_tcgen05_page_ok(page)):
-                _check(kernel.de_shared_tcgen05(*work, *after), "shared prefix attention (tcgen05)")
+                _check(kernel.de_shared_tcgen05(*work, plan.turns, *after),
+                       "shared prefix attention (tcgen05)")
             elif name.startswith("f32") and pages_fit:
                 _check(library.load("shared_prefix_f32").de_shared_f32(*work, rows, order, *after),
                        "shared prefix attention (float32)")
