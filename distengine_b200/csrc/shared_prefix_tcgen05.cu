@@ -8,18 +8,22 @@
 //     partial result of its own, so that one's exponentials run beside the other's products here too.
 // Warps:
 //   * warps 0-7 and 8-15 are the pipelines' softmax threads, two threads a row (= a lane of tensor
-//     memory), each 32 keys of either half of a tile: 64 scores into registers, exponentials in float32, weights as
-//     bfloat16 back into tensor memory as the A operand of the second product;
+//     memory), each 32 keys of each half of a tile: scores into registers, exponentials in float32, weights
+//     back into tensor memory as the A operand of the second product, which takes bfloat16 (half a step of
+//     2^-8 a weight; the sum is of the weights before they are rounded);
 //   * warps 16 and 17, one thread each, issue a pipeline's s = q k^T (operands in shared memory) and
 //     o += p v (p in tensor memory, v MN-major straight from the pages);
-//   * warp 18 (and 19) fetch: a ring of buffers of 128 keys or 128 values, one TMA box a page and 64 features.
-// A row's exponentials refer to a maximum that is raised, and o rescaled, only when a score has grown by
-// more than 2^8 beyond it.
+//   * warps 18 and 19 fetch: a ring of buffers of 128 keys or 128 values, one TMA box a page and 64 features.
+// A tile goes through in halves of 64 keys, each with columns of tensor memory of its own, so a half's scores
+// are formed while the other's exponentials are (512 rows behind 65,003 keys 151 us; tiles of 128 keys at a
+// time, whose scores had to wait for the weights over them, 171).  A row's exponentials refer to a maximum
+// that is raised, and o rescaled, only when a score has grown by more than 2^8 beyond it.
 //
 // What bounds it: with r rows a block a byte of keys and values takes r multiply-adds, so up to 128 rows
-// it is the cache's way from memory (at head size 128), beyond it the tensor cores and, as much, the
-// exponentials: a tile of 128 x 128 scores takes the tensor cores 1,024 cycles at head size 128 and 512
-// at 64, its exponentials 1,024 (16 a cycle).
+// it is the cache's way from memory (at head size 128: 108 rows behind 15,566 keys of 32 kv heads, 255 MB, 53 us
+// of the call's 76), beyond it the tensor cores and, as much, the exponentials: 128 x 128 scores take the
+// tensor cores 1,024 cycles at head size 128 and 512 at 64, their exponentials 1,024 (16 a cycle); 512 rows
+// behind 65,003 keys run at 880 TFLOP/s.
 //
 // Every wait is bounded (status 3; the block then stores no result, runs to its end and frees its tensor
 // memory).  One block an SM.
@@ -49,11 +53,9 @@ constexpr int SUB = 128 * 128;                // bytes of a sub-tile: 128 rows o
 constexpr int BUFFER = KS * SUB;              // 128 keys, or their values
 constexpr int BUFFERS = D == 64 ? 10 : 5;     // what shared memory has room for beside q
 constexpr int SOFTMAX_WARPS = 16, MMA_WARP = 16, COPY_WARP = 18;
-// Where the pipelines take turns, two warps fetch: one issues a box in some 100 cycles, too slowly for small
-// pages (108 rows behind 15,566 keys in pages of 16: 92 us, with two 77; in pages of 128 83 and 71).
-// Elsewhere one keeps up (512 rows behind 65,003 keys: 170 us, with two 178).
-template <bool TURNS> __host__ __device__ constexpr int copy_warps() { return TURNS ? 2 : 1; }
-template <bool TURNS> __host__ __device__ constexpr int threads() { return (COPY_WARP + copy_warps<TURNS>()) * 32; }
+// Two warps fetch: one issues a box in some 100 cycles, too slowly for small pages (108 rows behind 15,566
+// keys in pages of 16: 92 us, with two 77; 512 rows behind 32,000 82.7 and 76.0, in pages of 128 75.9 and 76.1).
+constexpr int COPY_WARPS = 2, THREADS = (COPY_WARP + COPY_WARPS) * 32;
 constexpr int SMEM = 2 * BUFFER + BUFFERS * BUFFER + 512 + 2 * 2 * LANES * 4;
 constexpr int COLUMNS = 512;
 // columns of tensor memory: scores of pipeline x and half h of a tile at 128 x + 64 h, weights over the first
@@ -222,9 +224,10 @@ template <bool B> struct Truth {
     static constexpr bool value = B;
 };
 
-// TURNS: there are items of up to 128 rows, whose tiles the pipelines take in turn
+// TURNS: there are items of up to 128 rows, whose tiles the pipelines take in turn (a form of its own: for
+// others 18 questions behind two documents take 40 us, with this form 43)
 template <bool TURNS>
-__global__ void __launch_bounds__(threads<TURNS>(), 1)
+__global__ void __launch_bounds__(THREADS, 1)
 shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
                       const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const int* __restrict__ block_table,
@@ -252,7 +255,6 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
     const int hk = blockIdx.x % kv_heads, g = heads / kv_heads;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool turns = TURNS && it.split != 0;            // the pipelines take the tiles in turn
-    constexpr int THREADS = threads<TURNS>(), COPIERS = copy_warps<TURNS>();
     const int n_tiles = (it.end - it.begin + KT - 1) / KT;
     const bool aligned = (smem_u32(smem_raw) & 1023u) == 0;
     if (!aligned && tid == 0) atomicExch(status, 4);
@@ -267,7 +269,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         mbar_init(&drained[0], 1);
         mbar_init(&drained[1], 1);
         for (int i = 0; i < BUFFERS; ++i) {
-            mbar_init(&full[i], COPIERS);
+            mbar_init(&full[i], COPY_WARPS);
             mbar_init(&empty[i], !turns && it.count > LANES ? 2 : 1);      // pipelines that read it
         }
         for (int x = 0; x < 4; ++x) {
@@ -337,7 +339,7 @@ shared_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
     if (warp >= COPY_WARP) {
         // ------------------------------------------------------------------ copies
         // unit 2 t: the keys of tile t, unit 2 t + 1: its values; the warps take the boxes in turn
-        const int w = warp - COPY_WARP, i = COPIERS * lane + w;
+        const int w = warp - COPY_WARP, i = COPY_WARPS * lane + w;
         int issued = 0;
         for (int t = 0; t < n_tiles; ++t) {
             const int key = it.begin + t * KT + i * box;
@@ -611,9 +613,8 @@ DE_EXPORT int de_shared_tcgen05(const void* q, int q_stride, const void* k_pages
     const auto kernel = turns ? shared_tcgen05_kernel<true> : shared_tcgen05_kernel<false>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return (int)e;
-    return de_launch(kernel, dim3((unsigned)num_items * kv_heads),
-                     dim3(turns ? threads<true>() : threads<false>()), SMEM, (cudaStream_t)stream,
-                     (const __nv_bfloat16*)q, q_stride, map_k, map_v, block_table, table_stride, num_pages,
+    return de_launch(kernel, dim3((unsigned)num_items * kv_heads), dim3(THREADS), SMEM,
+                     (cudaStream_t)stream, (const __nv_bfloat16*)q, q_stride, map_k, map_v, block_table, table_stride, num_pages,
                      seq_slot, (const Item*)items, partial_acc, (float2*)partial_ml, heads, kv_heads, page,
                      scale, status);
 }
