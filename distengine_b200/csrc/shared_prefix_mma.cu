@@ -11,6 +11,8 @@
 // A row's exponentials refer to a maximum that is raised only when a score has grown by more than 2^8
 // beyond it (the quotient does not depend on it), so most tiles need no exchange between lanes and no
 // rescaling of the results.
+// Weights enter the second product as bfloat16, which its operands are (half a step of 2^-8 each); their sum is
+// of the float32 ones.
 
 #include "shared_prefix.cuh"
 
