@@ -3,9 +3,10 @@
 //
 // A block of 128 threads takes 8, 16 or 32 query rows with a range of keys, in tiles of 64.  Both products
 // are tiled in registers: a thread has ROWS / 8 rows and, of the scores, four keys, of the results, four
-// features in 64, so that a shared-memory read of 16 bytes feeds up to 16 multiply-adds.  With r rows a
-// key's element is read once from memory for r multiply-adds; from about 22 rows on the multiply-adds
-// are what bounds it (72 TFLOP/s against 6.55 TB/s), below it the cache's way from memory.  The keys of
+// features in 64.  With r rows a key's element is read once from memory for r multiply-adds: few rows wait for
+// the cache (4 rows behind 2,001 keys of 32 kv heads, 66 MB, 34 us), many for shared memory, whose 16-byte reads
+// take four cycles of its pipe whoever shares their addresses: eight for 64 multiply-adds of the first product
+// (160 rows a group behind 1,656 keys of 8 kv heads of 128, twice: 141 us, 15 TFLOP/s).  The keys of
 // the next tile are copied while the values are at work and the next values while the keys are.
 
 #include "shared_prefix.cuh"
