@@ -305,8 +305,8 @@ int rows_of(const void* q, int q_stride, const void* k_pages, const void* v_page
         if (e != cudaSuccess) return (int)e;
     }
     return de_launch(shared_rows_kernel<T>, dim3((unsigned)num_items * kv_heads, (tile_rows + ROWS - 1) / ROWS),
-                     dim3(THREADS), smem, stream, (const T*)q, q_stride, (const T*)k_pages, (const T*)v_pages, block_table,
-                     table_stride, num_pages, seq_slot, seq_pos0, (const Item*)items, partial_acc,
+                     dim3(THREADS), smem, stream, (const T*)q, q_stride, (const T*)k_pages,
+                     (const T*)v_pages, block_table, table_stride, num_pages, seq_slot, seq_pos0, (const Item*)items, partial_acc,
                      (float2*)partial_ml, heads, kv_heads, d, page, scale, unit, order, status);
 }
 
@@ -327,8 +327,8 @@ DE_EXPORT int de_shared_rows(int dtype, const void* q, int q_stride, const void*
         return -2;
     const auto f = dtype == DE_F32 ? rows_of<float> : rows_of<__nv_bfloat16>;
     return f(q, q_stride, k_pages, v_pages, block_table, table_stride, num_pages, seq_slot, seq_pos0,
-             items, num_items, tile_rows, unit, order, partial_acc, partial_ml, heads, kv_heads, head_dim, page, scale, status,
-             (cudaStream_t)stream);
+             items, num_items, tile_rows, unit, order, partial_acc, partial_ml, heads, kv_heads,
+             head_dim, page, scale, status, (cudaStream_t)stream);
 }
 
 // `most`: partial results of a row, at most (up to 1,024).

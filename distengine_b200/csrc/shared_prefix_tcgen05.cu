@@ -614,7 +614,7 @@ DE_EXPORT int de_shared_tcgen05(const void* q, int q_stride, const void* k_pages
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return (int)e;
     return de_launch(kernel, dim3((unsigned)num_items * kv_heads), dim3(THREADS), SMEM,
-                     (cudaStream_t)stream, (const __nv_bfloat16*)q, q_stride, map_k, map_v, block_table, table_stride, num_pages,
-                     seq_slot, (const Item*)items, partial_acc, (float2*)partial_ml, heads, kv_heads, page,
+                     (cudaStream_t)stream, (const __nv_bfloat16*)q, q_stride, map_k, map_v,
+                     block_table, table_stride, num_pages, seq_slot, (const Item*)items, partial_acc, (float2*)partial_ml, heads, kv_heads, page,
                      scale, status);
 }

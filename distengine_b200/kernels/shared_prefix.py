@@ -116,8 +116,9 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
     """``seq_qlen``: tokens that each request brings; ``group_sizes``: how many requests, in their
     order, share a prefix; ``prefix_lens``: its keys (0: they share nothing); ``group``: query heads a
     kv head.  ``prefix_tile``: (rows, keys) -> ``Tile`` for a group of that many rows and its prefix;
-    ``own_tile`` the same for one request's own keys.  ``tail``: about how many keys of its own a request has at most (how
-    many ranges they are cut into goes by it, not which keys are seen)."""
+    ``own_tile`` the same for one request's own keys.  ``tail``: about how many keys of
+    its own a request has at most (how many ranges they are cut into goes by it, not which keys are
+    seen)."""
     qlen = np.asarray(seq_qlen, dtype=np.int64).reshape(-1)
     sizes = np.asarray(group_sizes, dtype=np.int64).reshape(-1)
     shared = np.asarray(prefix_lens, dtype=np.int64).reshape(-1)
@@ -267,8 +268,9 @@ class SharedPrefixAttention:
             # 55.5 and 39.7; 20 rows behind 2,040 of 8 17.9 and 18.7; 37 rows behind 6,373 of 32 40.6 and,
             # three tiles, 44.2; 48 rows behind 1,214 of 4, head size 64, 16.0 and 12.5)
             if rows > 32 and wide:
-                return (Tile("tcgen05", 128, 128, sms, 2, least=256, overhead=512, own_key=self.head_dim / 256) if rows <= 128 else
-                        Tile("tcgen05", 256, 128, sms, overhead=512, own_key=self.head_dim / 256))
+                costs = {"overhead": 512, "own_key": self.head_dim / 256}
+                return (Tile("tcgen05", 128, 128, sms, 2, least=256, **costs) if rows <= 128 else
+                        Tile("tcgen05", 256, 128, sms, **costs))
             return few
 
         return shared, lambda rows, keys: few
