@@ -31,9 +31,12 @@ constexpr int MAX_VOCAB = 1 << 27;
 // Which of two beams' candidates comes first depends on both rows' sums, and sums of float32
 // exponentials are off by some 1e-7: `slices` forms them so (a 64-bit sum of groups of 16), and
 // `join` compares with them only what is further apart than such sums can be wrong.  Where two
-// neighbours in its order are nearer than that (one selection of a thousand, or beams with equal
-// rows), it forms the sums of their rows again in 64 bits, as integers, so that the order of a row's
-// tokens does not matter, and orders again.
+// neighbours in its order are nearer than that, or the last one taken and any candidate of another
+// beam (one selection of a thousand, or beams with equal rows), it forms the sums of their rows again
+// in 64 bits, as integers, so that the order of a row's tokens does not matter, and orders again.
+// That is enough: a row's own candidates are in their order whatever its sum; whoever is in its wrong
+// place against the last one taken is of another beam and near it; and between two of those taken
+// that are the wrong way round all neighbours are near, and some of other beams.
 //
 // How far a fast sum may be off, relative to itself: ex2.approx 2^-22; its argument, a number of up to
 // 25 below the largest, rounded to half a step of 2^-20 for the smallest terms, which can have half of
@@ -94,24 +97,16 @@ __device__ __forceinline__ float exponent_of(float top) {
 
 // A threshold with which `count(t)`, the number of keys of at least t over the block, lies between
 // `want` and `most`, or all keys but 0 where there are at most `most`.  `low` is a guess from below
-// (1: none), `lower()` another where the first leaves too few, `top` the largest key; the range between is
-// halved until it is met, which distinct keys guarantee for most >= want (keys that are the same end
-// with the largest threshold that has `want`).  `count` and `lower` are called by all threads.
-template <typename Count, typename Lower>
-__device__ __forceinline__ u64 threshold(u64 low, Lower lower, u64 top, int want, int most, Count count) {
+// (1: none), `top` the largest key; the range between is halved until it is met, which distinct keys
+// guarantee for most >= want (keys that are the same end with the largest threshold that has `want`).
+// `count` is called by all threads.
+template <typename Count>
+__device__ __forceinline__ u64 threshold(u64 low, u64 top, int want, int most, Count count) {
     u64 high = top;
     if (low > 1) {
-        int n = count(low);
+        const int n = count(low);
         if (n >= want && n <= most) return low;
-        if (n < want) {
-            high = low - 1;
-            low = lower();
-            if (low > 1) {
-                n = count(low);
-                if (n >= want && n <= most) return low;
-                if (n < want) { high = low - 1; low = 1; }
-            }
-        }
+        if (n < want) { high = low - 1; low = 1; }
     }
     if (low <= 1) {
         if (top == 0 || count(1) <= most) return 1;
@@ -325,9 +320,8 @@ beam_slices_kernel(const float* __restrict__ logits, long long stride, int vocab
         if (tid == 0) counts_s[turn == 2 ? 0 : turn + 1] = 0;
         return k;
     };
-    const u64 last = threshold(guess > NOTHING ? (u64)guess << 32 : 1, [] { return (u64)1; },
-                               (u64)top << 32 | 0xffffffffu, take, min(max(6 * take, 96), WINNERS),
-                               segments_from);
+    const u64 last = threshold(guess > NOTHING ? (u64)guess << 32 : 1, (u64)top << 32 | 0xffffffffu, take,
+                               min(max(6 * take, 96), WINNERS), segments_from);
     if (tid == 0) winners_s = 0;
     __syncthreads();
     for (int i = tid; i < segments; i += SLICE_THREADS)
@@ -425,7 +419,7 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
     __shared__ double max_s[MAX_BEAMS], log_s[MAX_BEAMS]; // log(sum exp) of a row: max + log
     __shared__ u64 warp_part[2][JOIN_THREADS / 32];
     __shared__ int counts_s[3];
-    __shared__ int pick_s[PICKS], order_s[MAX_TAKE + 1];
+    __shared__ int pick_s[PICKS], order_s[MAX_TAKE];
     __shared__ u64 pick_total_s[PICKS];
     __shared__ float score_s[MAX_BEAMS];
     __shared__ int count_s;
@@ -493,8 +487,7 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
                (unsigned)key_token(k);
     };
     asm volatile("cp.async.wait_all;\n" ::: "memory");
-    // one more than is taken: what the last one taken is compared with
-    const int want = take + 1, most = max(2 * want, 96);
+    const int most = max(2 * take, 96);
     unsigned formed = 0;                                  // rows whose sums are 64-bit ones
     int found;
     for (;;) {
@@ -534,8 +527,8 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
                 }
             }
         } else {
-            // the largest, and a guess at the last one wanted: the largest last one of a slice, of which
-            // there is one more than are wanted unless they are all in that slice; then the next largest
+            // the largest, and a guess at the last one taken: the largest last one of a slice, which has
+            // as many as are taken that are no smaller
             u64 top = 0, guess = 0;
             for (int c = tid; c < n; c += JOIN_THREADS) {
                 const u64 t = key_s[c] ? total_key(total_of(c)) : 0;
@@ -556,19 +549,7 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
             }
 
             // the best by their totals; of those with the total of the last place the first by `place`
-            auto next = [&] {
-                u64 v = 0;
-                for (int i = tid; i < beams * slices; i += JOIN_THREADS) {
-                    const int c = i * take + take - 1;
-                    if (key_s[c] && total_s[c] < guess) v = max(v, total_s[c]);
-                }
-                v = warp_largest(v);
-                if (lane == 0) warp_part[0][warp] = v;
-                __syncthreads();
-                for (int w = 0; w < JOIN_THREADS / 32; ++w) v = max(v, warp_part[0][w]);
-                return max(v, (u64)1);
-            };
-            const u64 t0 = threshold(guess, next, top, want, most, [&](u64 t) {
+            const u64 t0 = threshold(guess, top, take, most, [&](u64 t) {
                 return over_block([&](int c) { return total_s[c] >= t; });
             });
             u64 last = ~0ull;
@@ -578,7 +559,7 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
                 while (low < high) {
                     const u64 mid = low + ((high - low) >> 1);
                     const int k = over_block([&](int c) { return total_s[c] == t0 && place(c) <= mid; });
-                    if (above + k >= want) high = mid; else low = mid + 1;
+                    if (above + k >= take) high = mid; else low = mid + 1;
                 }
                 last = high;
             }
@@ -597,18 +578,22 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
             const u64 x = pick_total_s[i], y = pick_total_s[j];
             return y > x || (y == x && place(pick_s[j]) < place(pick_s[i]));
         }, [&](int i, int rank) {
-            if (rank < want) order_s[rank] = pick_s[i];
+            if (rank < take) order_s[rank] = pick_s[i];
         });
         __syncthreads();
-        found = min(found, want);
-        // neighbours of different beams that are too near each other for the sums that they have
-        if (tid + 1 < found) {
-            const int c = order_s[tid], d = order_s[tid + 1];
-            const unsigned rows = 1u << (c / per_beam) | 1u << (d / per_beam);
+        found = min(found, take);
+        // candidates of different beams that are too near each other for the sums that they have
+        auto compare = [&](int c, int d) {
+            const int b = c / per_beam, e = d / per_beam;
+            const unsigned rows = 1u << b | 1u << e;
             const double a = key_total(total_s[c]), z = key_total(total_s[d]);
-            if (c / per_beam != d / per_beam && (rows & ~formed) && a < INFINITY && a - z <= UNSURE)
+            if (b != e && (rows & ~formed) && fabs(a) < INFINITY && fabs(a - z) <= UNSURE)
                 atomicOr(&again_s, rows);
-        }
+        };
+        if (tid + 1 < found) compare(order_s[tid], order_s[tid + 1]);
+        if (found == take)
+            for (int c = tid; c < n; c += JOIN_THREADS)
+                if (total_s[c]) compare(order_s[take - 1], c);
         __syncthreads();
         if (!(again_s & ~formed)) break;
     }

@@ -162,6 +162,29 @@ def test_nearly_equal_totals(gap, vocabulary):
         _check(logits, torch.full((2, 4), -1.0), 8)
 
 
+@pytest.mark.parametrize("vocabulary", [517, 32001, 50021, 128257])
+@pytest.mark.parametrize("take", [1, 2, 5])
+def test_the_last_place_among_equal_totals(vocabulary, take):
+    """Two beams with one row, in which more tokens are equal than are taken: the lower beam has every place,
+    also where the other one's sum comes out larger and its tokens would fill the list."""
+    g = torch.Generator().manual_seed(vocabulary + take)
+    for _ in range(3):
+        row = torch.randn(6, vocabulary, generator=g) * 2
+        for r in row:
+            r[torch.randperm(vocabulary, generator=g)[: take + 2]] = float(r.max()) + 1.0
+        _check(row.repeat_interleave(2, 0), torch.full((6, 2), -1.0), take)
+
+
+@pytest.mark.parametrize("take", [1, 2, 3, 9])
+def test_the_last_place_among_many_beams(take):
+    """Eight beams whose best totals are nearly equal: whoever has the last place is compared with all."""
+    g = torch.Generator().manual_seed(take)
+    for vocabulary in (300, 32001):
+        logits = torch.randn(96, vocabulary, generator=g) * 2
+        top = torch.log_softmax(logits.double(), 1).amax(1).view(12, 8)
+        _check(logits, (-3.0 - top).float(), take)
+
+
 def test_streams_and_graphs():
     """Two captured selections replayed side by side."""
     from distengine_b200.kernels import ops
