@@ -32,8 +32,9 @@ constexpr int MAX_VOCAB = 1 << 27;
 // exponentials are off by some 1e-7: `slices` forms them so (a 64-bit sum of groups of 16), and
 // `join` compares with them only what is further apart than such sums can be wrong.  Where two
 // neighbours in its order are nearer than that, or the last one taken and any candidate of another
-// beam (one selection of a thousand, or beams with equal rows), it forms the sums of their rows again
-// in 64 bits, as integers, so that the order of a row's tokens does not matter, and orders again.
+// beam (one selection of a thousand, or beams with equal rows), it forms the sums of their rows again,
+// as whole numbers of 2^-68 in two words, so that the order of a row's tokens does not matter and the
+// smallest terms count (2^27 of them are off by 2^-42 together), and orders again.
 // That is enough: a row's own candidates are in their order whatever its sum; whoever is in its wrong
 // place against the last one taken is of another beam and near it; and between two of those taken
 // that are the wrong way round all neighbours are near, and some of other beams.
@@ -497,22 +498,31 @@ beam_join_kernel(const float* __restrict__ logits, long long stride, int vocab,
         formed |= again;
         for (int b = 0; b < beams; ++b) {
             if (!(again >> b & 1)) continue;
-            // terms of up to 1 as whole numbers of 2^-scale, whose sum fits 63 bits
-            const int scale = min(46, 62 - (32 - __clz(vocab)));
-            const double unit = __hiloint2double((1023 + scale) << 20, 0);
+            // a term, of up to 1, as a whole number of 2^-34 and what is left of it of 2^-68: sums of up to
+            // 2^27 of either fit 62 bits
+            constexpr double UNIT = 17179869184.0;        // 2^34
             const float* x = logits + ((long long)g * beams + b) * stride;
             const double m = max_s[b];
-            u64 sum = 0;
-            for (int i = tid; i < vocab; i += JOIN_THREADS)
-                sum += (u64)__double2ll_rn(exp((double)x[i] - m) * unit);
+            u64 high = 0, low = 0;
+            for (int i = tid; i < vocab; i += JOIN_THREADS) {
+                const double e = exp((double)x[i] - m) * UNIT, whole = floor(e);
+                high += (u64)__double2ll_rn(whole);
+                low += (u64)__double2ll_rn((e - whole) * UNIT);
+            }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane == 0) warp_part[0][warp] = sum;
+            for (int o = 16; o > 0; o >>= 1) {
+                high += __shfl_xor_sync(0xffffffffu, high, o);
+                low += __shfl_xor_sync(0xffffffffu, low, o);
+            }
+            if (lane == 0) { warp_part[0][warp] = high; warp_part[1][warp] = low; }
             __syncthreads();
             if (tid == 0) {
-                sum = 0;
-                for (int w = 0; w < JOIN_THREADS / 32; ++w) sum += warp_part[0][w];
-                log_s[b] = log((double)sum / unit);
+                high = low = 0;
+                for (int w = 0; w < JOIN_THREADS / 32; ++w) {
+                    high += warp_part[0][w];
+                    low += warp_part[1][w];
+                }
+                log_s[b] = log(((double)high + (double)low / UNIT) / UNIT);
             }
             __syncthreads();
         }

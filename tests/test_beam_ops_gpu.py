@@ -185,6 +185,24 @@ def test_the_last_place_among_many_beams(take):
         _check(logits, (-3.0 - top).float(), take)
 
 
+@pytest.mark.parametrize("vocabulary", [5000, 128256, 1 << 20, 1 << 24])
+@pytest.mark.parametrize("part", [0.5, 0.99, 1.01, 1.5])
+def test_nearly_equal_totals_of_peaked_rows(vocabulary, part):
+    """A token that has nearly all and, behind it, very many that have next to nothing: together they are what
+    decides.  One beam's total is ``part`` of their weight above, less that weight; the other's is 0."""
+    bits = vocabulary.bit_length()
+    for least in (bits - 64.0, bits - 63.1, -46.1):              # logarithms to base 2 of one token's weight
+        logits = torch.full((2, vocabulary), -200.0)
+        logits[0] = least * math.log(2.0)
+        logits[:, vocabulary // 3] = 0.0
+        weight = math.log1p((vocabulary - 1) * math.exp(float(logits[0, 0])))
+        scores = torch.tensor([[part * weight, 0.0]], dtype=torch.float32)
+        assert weight < 1e-4 and abs(float(scores[0, 0]) / weight - part) < 1e-6
+        _, beam, token = _select(logits.to(DEV), scores.to(DEV), 1)
+        assert token.tolist() == [[vocabulary // 3]]
+        assert beam.tolist() == [[0 if part > 1.0 else 1]], (least, weight)
+
+
 def test_streams_and_graphs():
     """Two captured selections replayed side by side."""
     from distengine_b200.kernels import ops
