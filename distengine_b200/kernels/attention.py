@@ -383,7 +383,7 @@ class AttentionLauncher:
         at = f"{self.key}/shared/"
         plan = SharedPlan({name: ctx.arrays[at + name] for name in names}, dict(shapes),
                           ctx.arrays[at + "seqs"], ctx.arrays[at + "token_seq"], partial_rows, most_parts,
-                          tokens, q.device, turns)
+                          tokens, q.device, turns, self.shared.group, self.shared.kv_heads)
         self.shared.run(q, out, k_pages, v_pages, block_table, ctx.seq_slot, ctx.seq_pos0, plan,
                         ctx.status, ctx.buffer)
 

@@ -30,9 +30,10 @@ class SharedPlan:
     """The work lists of a step's requests: ``items`` by kernel, int32 [n, 8] (``shared_prefix::Item``;
     ``shapes``: their most rows and the unit of their ranges), ``seqs`` int32 [requests, 8]
     (``shared_prefix::Joined``), ``token_seq`` int32 [tokens]; ``partial_rows`` rows of partial results, at
-    most ``most_parts`` of one row; ``turns``: some items leave two.  The arrays are numpy's until ``to``
-    moves them.  (Kernels read them before the kernel in front of theirs has ended: on the device they come
-    from copies, as ``to`` and a step's upload make them.)"""
+    most ``most_parts`` of one row; ``turns``: some items leave two.  ``group`` query heads a kv head and
+    ``kv_heads`` are what the items' rows count: a plan is for layers with these.  The arrays are numpy's
+    until ``to`` moves them.  (Kernels read them before the kernel in front of theirs has ended: on the
+    device they come from copies, as ``to`` and a step's upload make them.)"""
     items: dict
     shapes: dict
     seqs: "np.ndarray | torch.Tensor"
@@ -42,13 +43,15 @@ class SharedPlan:
     tokens: int
     device: "torch.device | None" = field(default=None)
     turns: bool = False
+    group: int = 0
+    kv_heads: int = 0
 
     def to(self, device: "torch.device | str") -> "SharedPlan":
         move = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(device)
         seqs = move(self.seqs)
         return SharedPlan({name: move(a) for name, a in self.items.items()}, self.shapes, seqs,
                           move(self.token_seq), self.partial_rows, self.most_parts, self.tokens, seqs.device,
-                          self.turns)
+                          self.turns, self.group, self.kv_heads)
 
 
 @dataclass(frozen=True)
@@ -212,7 +215,8 @@ def plan_shared(seq_qlen, group_sizes, prefix_lens, group: int, kv_heads: int, p
     return SharedPlan({name: np.concatenate(items[name]) for name in names}, shapes, seqs,
                       np.repeat(np.arange(len(qlen)), qlen), base,
                       int((seqs[:, 3] + seqs[:, 6]).max(initial=0)), total,
-                      turns=any(t.places > 1 for members in by_name.values() for _, t in members))
+                      turns=any(t.places > 1 for members in by_name.values() for _, t in members),
+                      group=group, kv_heads=kv_heads)
 
 
 class SharedPrefixAttention:
@@ -294,7 +298,8 @@ class SharedPrefixAttention:
             block_table: torch.Tensor, seq_slot: torch.Tensor, seq_pos0: torch.Tensor,
             plan: SharedPlan, status: "torch.Tensor | None" = None, buffer=None) -> None:
         """q: a row a token, [heads * d] query features at its front (row stride free), requests in
-        the plan's order; out [tokens, heads * d] (row stride free); keys and values [pages,
+        the plan's order (``plan``: of any layer with as many heads and kv heads); out
+        [tokens, heads * d] (row stride free); keys and values [pages,
         kv_heads, page, d], this step's tokens' among them; ``block_table`` [slots, max pages] int32.
         ``seq_slot`` int32: each request's row of the table; the first of a group has the pages of
         the prefix, all have those of their own keys.  ``seq_pos0`` int32: position of each request's
@@ -302,6 +307,9 @@ class SharedPrefixAttention:
         key without a page is not seen and sets ``status`` to 2.  ``buffer(name, shape, dtype)``:
         where the partial results lie during the call (None: fresh memory)."""
         d, heads, kv_heads, tokens = self.head_dim, self.heads, self.kv_heads, plan.tokens
+        _need(plan.group == self.group and plan.kv_heads == kv_heads,
+              f"shared prefix: the plan is one for {plan.kv_heads} kv heads of {plan.group} query heads "
+              f"each, the layer has {kv_heads} of {self.group}")
         _need(q.dim() == out.dim() == 2, "shared prefix: q and out have a row a token of the plan")
         _need(k_pages.dim() == 4, "shared prefix: pages must be [pages, kv_heads, page, head_dim]")
         q_shape, (q_stride, q_one) = q.shape, q.stride()
@@ -336,10 +344,12 @@ class SharedPrefixAttention:
         lib = library.load("shared_prefix")
         tag, stream = _tag(self.dtype), _stream()
         q_at, k_at, v_at = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
-        # what a kernel copies in pieces has to lie so; the next one in this list takes it otherwise
+        # what a kernel copies in pieces has to lie so; the next one in this list takes it otherwise, and
+        # what a plan of another type or head size has for kernels that this layer does not have
         pages_fit = not (k_at % 16 or v_at % 16)
-        aligned = pages_fit and not (q_stride % 2 or q_at % 4)
-        wide = pages_fit and not (q_stride % 8 or q_at % 16)
+        rows_fit = pages_fit and self.dtype == torch.float32 and d % 4 == 0
+        aligned = pages_fit and self.tensor_cores and not (q_stride % 2 or q_at % 4)
+        wide = pages_fit and self.tcgen05_module is not None and not (q_stride % 8 or q_at % 16)
         before = (q_at, q_stride, k_at, v_at, block_table.data_ptr(), block_table.stride(0), pages,
                   seq_slot.data_ptr(), seq_pos0.data_ptr())
         after = (acc, ml, heads, kv_heads, d, page, self.scale, status.data_ptr(), stream)
@@ -352,7 +362,7 @@ class SharedPrefixAttention:
                     and (kernel := library.load(*self.tcgen05_module)).de_shared_tcgen05_page_ok(page)):
                 _check(kernel.de_shared_tcgen05(*work, plan.turns, *after),
                        "shared prefix attention (tcgen05)")
-            elif name.startswith("f32") and pages_fit:
+            elif name.startswith("f32") and rows_fit:
                 _check(library.load("shared_prefix_f32").de_shared_f32(*work, rows, order, *after),
                        "shared prefix attention (float32)")
             elif name in ("warp", "tcgen05") and aligned:

@@ -169,3 +169,22 @@ def test_a_call_off_the_current_device_is_refused():
                        lambda r, k: TILES["one"][0])
     with pytest.raises(ValueError, match="not on the device"):
         _call(plan=plan)
+
+
+@pytest.mark.parametrize("group,kv_heads", [(4, 2), (2, 4), (1, 2), (4, 1)])
+def test_a_plan_for_other_heads_is_refused(group, kv_heads):
+    """Its rows would lie outside q."""
+    from distengine_b200.kernels.shared_prefix import SharedPlan
+    tile = TILES["one"][0]
+    plan = plan_shared([1, 1], [2], [16], group, kv_heads, lambda r, k: tile, lambda r, k: tile)
+    with pytest.raises(ValueError, match="shared prefix: the plan"):
+        _call(plan=plan.to("cpu"))
+    with pytest.raises(ValueError, match="shared prefix: the plan"):
+        _call(plan=SharedPlan(plan.items, plan.shapes, plan.seqs, plan.token_seq, plan.partial_rows,
+                              plan.most_parts, plan.tokens).to("cpu"))
+
+
+def test_a_plan_keeps_its_heads():
+    tile = TILES["places"][0]
+    plan = plan_shared([1, 1], [2], [16], 5, 3, lambda r, k: tile, lambda r, k: tile).to("cpu")
+    assert (plan.group, plan.kv_heads, plan.turns) == (5, 3, True)

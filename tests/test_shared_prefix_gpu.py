@@ -181,6 +181,19 @@ def test_a_plan_holds_from_step_to_step(dtype):
              dtype, seed=own).check(layer=layer, plan=plan)
 
 
+@pytest.mark.parametrize("made,used", [((torch.float32, 64), (torch.bfloat16, 64)),
+                                       ((torch.bfloat16, 64), (torch.float32, 64)),
+                                       ((torch.bfloat16, 128), (torch.bfloat16, 32)),
+                                       ((torch.bfloat16, 128), (torch.bfloat16, 6)),
+                                       ((torch.float32, 64), (torch.float32, 6))])
+def test_a_plan_of_another_type_or_head_size(made, used):
+    """It names kernels that the layer does not have: others do their work."""
+    (dtype, d), groups = used, GROUPS["many"] + GROUPS["portions"]
+    case = Case(groups, 8, 2, d, 16, dtype, seed=50)
+    layer = _layer(made[0], 8, 2, made[1], 0.1)
+    case.check(plan=layer.plan(case.qlen, case.sizes, case.prefix, 100))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_sharing_changes_no_request(dtype):
     """A request's result is the same, but for the order of the sums, whoever else is in its group."""
