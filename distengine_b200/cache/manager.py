@@ -218,6 +218,9 @@ class CacheManager:
             sgroup.state = torch.zeros((len(sgroup.entries), max_seqs, *sgroup.spec.shape),
                                        dtype=sgroup.spec.dtype, device=self.device)
         self._reads = list(reads_cache_of)
+        # the device word in which kernels of the cache's own moves record what they skipped (a step
+        # runner gives its own, which it looks at); None: the operators' (``ops.take_status``)
+        self.status: "torch.Tensor | None" = None
         # block-table rows travel through a pinned buffer of the manager's own: the host rows may
         # change again (a release, the next reserve) while an earlier upload is still queued
         self._stage: "torch.Tensor | None" = None
@@ -503,7 +506,7 @@ class CacheManager:
                 from ..kernels import ops
                 rows = torch.tensor(slots, dtype=torch.int32).to(self.device)
                 for tensor in tensors:
-                    ops.beam_reorder(tensor, rows, parent)
+                    ops.beam_reorder(tensor, rows, parent, self.status)
                 return
             to = [(s, row[p]) for row, source in zip(slots, parents) for s, p in zip(row, source) if s >= 0]
             for tensor in tensors:                        # (tests of the host side)

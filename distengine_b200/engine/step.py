@@ -71,6 +71,7 @@ class StepRunner:
         self.workspace = Workspace(self.device)
         self.status = (status if status is not None
                        else torch.zeros(1, dtype=torch.int32, device=self.device))
+        cache.status = self.status                           # of what the cache moves on the device
         self._host_meta: "torch.Tensor | None" = None        # pinned int32 staging
         self._dev_meta: "torch.Tensor | None" = None
         self._uploaded = torch.cuda.Event()

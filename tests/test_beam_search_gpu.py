@@ -152,6 +152,23 @@ def test_graphs_change_nothing(model_root, monkeypatch):
     assert [h.score for h in found[0]] == [h.score for h in found[1]]
 
 
+def test_a_move_that_could_not_be_made_raises(model_root):
+    """What the cache's own moves on the device report goes to the word that the engine looks at."""
+    from distengine_b200.engine.step import KernelStatusError, StepEntry
+    folder, _ = _llama("tiny_a", model_root)
+    engine = _engine(folder, "float32", block_size=16, num_blocks=16, decode_batch_size=4)
+    prompt = tiny_configs.prompt_tokens("tiny_a", 10, 1)
+    engine.runner.step([StepEntry("a", prompt, [9])])
+    engine.cache.fork("a", ["b"])
+    engine.runner.check_status()
+    engine.cache._move([["a", "a"]], [[1, 0]])            # (no caller can ask for this)
+    with pytest.raises(KernelStatusError, match="status 5"):
+        engine.runner.check_status()
+    engine.runner.check_status()
+    engine.cache.release("a"), engine.cache.release("b")
+    assert len(engine.beam_search([prompt], 3, 2)[0]) == 2
+
+
 def test_entry_points_and_refusals(model_root):
     from distengine_b200 import generate_beam
     folder, _ = _llama("tiny_a", model_root)
