@@ -91,15 +91,35 @@ _status_words: dict[torch.device, torch.Tensor] = {}
 
 
 def _status_word(status: "torch.Tensor | None", like: torch.Tensor) -> torch.Tensor:
-    """The word in which a kernel records what it skipped: the caller's, or one of the device's."""
+    """The word in which a kernel records what it skipped: the caller's, or one of the device's
+    (``take_status``)."""
     if status is not None:
         _need(status.dtype == torch.int32 and status.numel() >= 1 and status.device == like.device,
               "status must be an int32 tensor on the operands' device")
         return status
     word = _status_words.get(like.device)
     if word is None:
-        word = _status_words[like.device] = torch.zeros(1, dtype=torch.int32, device=like.device)
+        word = torch.zeros(1, dtype=torch.int32, device=like.device)
+        # (one that is made while a graph is captured would be zeroed at every replay: it is the call's own)
+        if not torch.cuda.is_current_stream_capturing():
+            _status_words[like.device] = word
     return word
+
+
+def take_status(device: "torch.device | str | int | None" = None) -> int:
+    """What kernels that were given no ``status`` word have recorded on the device (None: the current one)
+    since the last call: 0, or a code whose meaning ``StepRunner.check_status`` has.  Waits for the current
+    stream.  A captured call that is the first on its device records nothing here: give it a word."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"status words are on CUDA devices, got {device}")
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    word = _status_words.get(device)
+    code = 0 if word is None else int(word.item())
+    if code:
+        word.zero_()
+    return code
 
 
 # ------------------------------------------------------------------------------- embedding
@@ -823,8 +843,8 @@ def beam_reorder(rows: torch.Tensor, slots: torch.Tensor, parent: torch.Tensor,
     rows [layers, pool, ...] contiguous, of any dtype (recurrent states, pages of a cache); slots int32
     [groups, beams]: each beam's row of the pool, all different (-1: a beam without one); parent int32
     [groups, beams]: a beam of the same group (-1: the row stays as it is); up to 32 beams.  What cannot be used
-    stays as it is and sets ``status`` to 5: a slot or parent outside its range, the parent's missing
-    row, all of a group of which a row is named twice."""
+    stays as it is and sets ``status`` (None: what ``take_status`` reads) to 5: a slot or parent outside its
+    range, the parent's missing row, all of a group of which a row is named twice."""
     _need(rows.dim() >= 2 and rows.is_contiguous(), "beam_reorder: rows [layers, pool, ...], contiguous")
     _need(slots.dim() == 2 and slots.shape == parent.shape and slots.shape[1] <= MAX_BEAMS
           and slots.dtype == parent.dtype == torch.int32 and slots.is_contiguous()

@@ -298,14 +298,15 @@ class SharedPrefixAttention:
             block_table: torch.Tensor, seq_slot: torch.Tensor, seq_pos0: torch.Tensor,
             plan: SharedPlan, status: "torch.Tensor | None" = None, buffer=None) -> None:
         """q: a row a token, [heads * d] query features at its front (row stride free), requests in
-        the plan's order (``plan``: of any layer with as many heads and kv heads); out
-        [tokens, heads * d] (row stride free); keys and values [pages,
-        kv_heads, page, d], this step's tokens' among them; ``block_table`` [slots, max pages] int32.
+        the plan's order (``plan``: of any layer with as many heads and kv heads); out [tokens, heads * d]
+        (row stride free); keys and values [pages, kv_heads, page, d], this step's tokens' among them;
+        ``block_table`` [slots, max pages] int32.
         ``seq_slot`` int32: each request's row of the table; the first of a group has the pages of
         the prefix, all have those of their own keys.  ``seq_pos0`` int32: position of each request's
         first token, not before the prefix's end.  A token sees the keys up to its own position; a
-        key without a page is not seen and sets ``status`` to 2.  ``buffer(name, shape, dtype)``:
-        where the partial results lie during the call (None: fresh memory)."""
+        key without a page is not seen and sets ``status`` (None: what ``ops.take_status`` reads) to 2; a
+        bounded wait that ran out sets it to 3.  ``buffer(name, shape, dtype)``: where the partial results
+        lie during the call (None: fresh memory)."""
         d, heads, kv_heads, tokens = self.head_dim, self.heads, self.kv_heads, plan.tokens
         _need(plan.group == self.group and plan.kv_heads == kv_heads,
               f"shared prefix: the plan is one for {plan.kv_heads} kv heads of {plan.group} query heads "

@@ -369,3 +369,35 @@ def test_large_rows_and_graphs():
         names[8], names[0], names[4] = taken
         for at in (0, 12_345_678, 29_999_999):
             assert rows[:, :, at].cpu().tolist() == [[9 * l + n for n in names] for l in range(5)]
+
+
+def test_the_status_of_calls_without_a_word():
+    """It is kept until it is read, also where the device's first such call was a captured one."""
+    from distengine_b200.kernels import ops
+    ops.take_status()
+    words, kept = ops._status_words, dict(ops._status_words)
+    rows = torch.randn(2, 12, 100, device=DEV)
+    slots = torch.tensor([[3, 12, 5]], dtype=torch.int32, device=DEV)
+    parent = torch.tensor([[1, 0, 0]], dtype=torch.int32, device=DEV)
+    stays = torch.arange(3, dtype=torch.int32, device=DEV)[None]
+    try:
+        words.clear()
+        assert ops.take_status() == 0
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.beam_reorder(rows, slots, stays)
+        graph.replay()
+        assert ops.take_status() == 0
+        ops.beam_reorder(rows, slots, parent)
+        graph.replay()
+        assert ops.take_status(DEV) == 5 and ops.take_status("cuda") == 0
+        with torch.cuda.graph(graph := torch.cuda.CUDAGraph()):
+            ops.beam_reorder(rows, slots, parent)
+        assert ops.take_status() == 0
+        graph.replay()
+        assert ops.take_status(torch.device(DEV)) == 5 and ops.take_status(0) == 0
+    finally:
+        words.clear()
+        words.update(kept)
+    with pytest.raises(ValueError, match="status"):
+        ops.take_status("cpu")
