@@ -683,7 +683,7 @@ beam_reorder_kernel(unsigned char* __restrict__ x, long long row_bytes, int pool
         bool bad = twice;
         if (tid < beams && !twice) {
             const int s = slot_s[tid], p = parent[g * beams + tid];
-            bad = s < -1 || s >= pool || p >= beams;
+            bad = s < -1 || s >= pool || p < -1 || p >= beams;
             if (!bad && s >= 0 && p >= 0 && p != tid) {
                 const int src = slot_s[p];
                 bad = src < 0 || src >= pool;

@@ -334,6 +334,16 @@ def test_what_cannot_be_moved_stays():
         assert status == 5 and torch.equal(device.cpu(), want), (slots, parent)
 
 
+def test_a_parent_below_minus_one_is_no_parent():
+    rows = torch.randn(2, 12, 100)
+    device = rows.to(DEV)
+    assert _reorder(device, torch.tensor([[3, 4, 5]], dtype=torch.int32),
+                    torch.tensor([[-2, 0, -1]], dtype=torch.int32)) == 5
+    want = rows.clone()
+    want[:, 4] = rows[:, 3]
+    assert torch.equal(device.cpu(), want)
+
+
 def test_refusals_of_the_reordering():
     from distengine_b200.kernels import ops
     i = lambda *shape: torch.zeros(*shape, dtype=torch.int32, device=DEV)
