@@ -90,13 +90,16 @@ class BeamSearch:
         if beams > cache.max_seqs:
             raise ValueError(f"{beams} beams are more than the {cache.max_seqs} requests that are live "
                              f"at a time (decode_batch_size)")
+        if beams > max_batch_tokens:
+            raise ValueError(f"{beams} beams are more than the {max_batch_tokens} tokens of a step "
+                             f"(max_batch_tokens)")
         if not isinstance(length_penalty, (int, float)) or length_penalty != length_penalty:
             raise ValueError("length_penalty must be a number")
         self.runner, self.cache, self.beams = runner, cache, beams
         self.max_batch_tokens, self.penalty = max_batch_tokens, float(length_penalty)
         # twice as many as beams: even if half of them end, there are enough that go on
         self.take = min(2 * beams, ops.MAX_TAKE)
-        self.groups = cache.max_seqs // beams
+        self.groups = min(cache.max_seqs, max_batch_tokens) // beams
         self.selector = BeamSelector(runner.device, self.groups, self.take)
 
     def _pages(self, prompt: "list[int]", max_new_tokens: int) -> int:
@@ -109,7 +112,7 @@ class BeamSearch:
     def run(self, prompts: "list[list[int]]", max_new_tokens: int, eos_token_id: int,
             name: str) -> "list[list[Hypothesis]]":
         """For every prompt its finished hypotheses, best first (up to ``beams``).  As many prompts at a
-        time as there are slots and pages for."""
+        time as there are slots and pages for, and tokens in a step."""
         have = self.cache.num_free_pages()
         for prompt in prompts:
             if self._pages(prompt, max_new_tokens) > have:

@@ -311,3 +311,31 @@ def test_a_prompt_that_cannot_fit_is_refused(monkeypatch):
     with pytest.raises(ValueError, match="pages"):
         search.run([[1] * 9], 8, -1, "t")
     assert not cache.live
+
+
+@pytest.mark.parametrize("beams,budget,groups", [(3, 8, 2), (3, 5, 1), (2, 2, 1), (1, 4, 4)])
+def test_a_step_keeps_to_the_token_budget(beams, budget, groups, monkeypatch):
+    monkeypatch.setattr(beam_module, "BeamSelector", _PlainSelector)
+    steps = []
+
+    class Runner(_ToyRunner):
+        def step(self, entries):
+            steps.append(sum(len(e.tokens) for e in entries))
+            return super().step(entries)
+
+    cache = _cache(pages=60, slots=9, specs=[PagedKVSpec(1, 1), StateSpec((2,))])
+    cache.poison = False
+    prompts = [[1, 2, 3, 4, 5, 6, 7, 8, 9], [4, 4], [9, 1, 2, 0], [5]]
+    search = BeamSearch(Runner(cache, 11, 17), cache, beams, budget)
+    assert search.groups == groups
+    found = search.run(prompts, 6, -1, "t")
+    assert max(steps) <= budget and beams * groups in steps
+    for prompt, got in zip(prompts, found):
+        want = plain_search(lambda ids: toy_logits(ids, 11, 17), prompt, beams, 6, -1, 1.0)
+        assert [h.token_ids for h in got] == [t for _, t in want]
+
+
+def test_more_beams_than_a_step_has_tokens_are_refused():
+    cache = _cache(pages=6, slots=8)
+    with pytest.raises(ValueError, match="max_batch_tokens"):
+        BeamSearch(_ToyRunner(cache, 11, 1), cache, 5, 4)
