@@ -17,6 +17,7 @@ The reference has no beam search; its nearest relative is ``generate_greedy_cach
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 
 from ..kernels import ops
@@ -93,8 +94,8 @@ class BeamSearch:
         if beams > max_batch_tokens:
             raise ValueError(f"{beams} beams are more than the {max_batch_tokens} tokens of a step "
                              f"(max_batch_tokens)")
-        if not isinstance(length_penalty, (int, float)) or length_penalty != length_penalty:
-            raise ValueError("length_penalty must be a number")
+        if not isinstance(length_penalty, (int, float)) or not abs(length_penalty) <= 1e300:
+            raise ValueError("length_penalty must be a finite number")
         self.runner, self.cache, self.beams = runner, cache, beams
         self.max_batch_tokens, self.penalty = max_batch_tokens, float(length_penalty)
         # twice as many as beams: even if half of them end, there are enough that go on
@@ -113,6 +114,9 @@ class BeamSearch:
             name: str) -> "list[list[Hypothesis]]":
         """For every prompt its finished hypotheses, best first (up to ``beams``).  As many prompts at a
         time as there are slots and pages for, and tokens in a step."""
+        # (scores of continuations of all lengths stay numbers: far within 1e308)
+        if abs(self.penalty) * math.log10(max(max_new_tokens, 2)) > 200.0:
+            raise ValueError(f"length_penalty {self.penalty} is too large for {max_new_tokens} tokens")
         have = self.cache.num_free_pages()
         for prompt in prompts:
             if self._pages(prompt, max_new_tokens) > have:

@@ -339,3 +339,16 @@ def test_more_beams_than_a_step_has_tokens_are_refused():
     cache = _cache(pages=6, slots=8)
     with pytest.raises(ValueError, match="max_batch_tokens"):
         BeamSearch(_ToyRunner(cache, 11, 1), cache, 5, 4)
+
+
+@pytest.mark.parametrize("penalty", [math.inf, -math.inf, 1e5, -1e5, 1e308, 10 ** 400])
+def test_length_penalties_beyond_the_number_range_are_refused(penalty, monkeypatch):
+    """A score is divided by the length to that power, which has to be a number above 0."""
+    monkeypatch.setattr(beam_module, "BeamSelector", _PlainSelector)
+    cache = _cache(pages=50, slots=4, specs=[PagedKVSpec(1, 1), StateSpec((2,))])
+    cache.poison = False
+    with pytest.raises(ValueError, match="length_penalty"):
+        BeamSearch(_ToyRunner(cache, 11, 1), cache, 2, 8, penalty).run([[1, 2]], 5, 3, "t")
+    assert not cache.live
+    found = BeamSearch(_ToyRunner(cache, 11, 1), cache, 2, 8, -3).run([[1, 2]], 5, 3, "t")
+    assert len(found[0]) == 2
