@@ -98,6 +98,67 @@ def test_llama_in_bfloat16(name, model_root, monkeypatch):
             assert abs(h.score - _score(logits_of, prompt, h.token_ids, 1.0)) <= 2 * 4e-2 * scale
 
 
+@pytest.mark.parametrize("name", ["tiny_d", "tiny_e"])
+@pytest.mark.parametrize("beams", [5, 12])
+@pytest.mark.parametrize("share", [True, False])
+def test_bfloat16_step_by_step(name, beams, share, model_root, monkeypatch):
+    """Every row of logits of a search is that of the sequence that its beam stands for, and the search over
+    these rows is the plain one: so the beams' contents, the keys that they share and the choice are all as
+    they should be.  (12 beams of three query heads a kv head: more than 32 rows behind the shared keys.)"""
+    from distengine_b200.kernels import attention
+    from gpu_helpers import BF16_MAX_REL
+    monkeypatch.setattr(attention, "SHARED_SAVES", 0 if share else 1 << 60)
+    folder, logits_of = _llama(name, model_root, torch.bfloat16)
+    prompt = tiny_configs.prompt_tokens(name, 70, 3)
+    engine = _engine(folder, "bfloat16", block_size=16, num_blocks=64, decode_batch_size=16)
+    held, rows, shared_steps = {}, {}, []
+    step, fork, reorder = engine.runner.step, engine.cache.fork, engine.cache.reorder
+
+    def follow_step(entries):
+        logits = step(entries)
+        at = 0
+        for e in entries:
+            held[e.request_id] = held.get(e.request_id, []) + e.tokens
+            for _ in e.want:
+                rows.setdefault(tuple(held[e.request_id]), logits[at].float().cpu())
+                at += 1
+        shared_steps.append(any("/shared/" in key for key in engine.runner.last_arrays))
+        return logits
+
+    def follow_fork(request_id, copies):
+        held.update({name: list(held[request_id]) for name in copies})
+        return fork(request_id, copies)
+
+    def follow_reorder(groups, parents):
+        for names, source in zip(groups, parents):
+            held.update(dict(zip(names, [held[names[p]] for p in source])))
+        return reorder(groups, parents)
+
+    monkeypatch.setattr(engine.runner, "step", follow_step)
+    monkeypatch.setattr(engine.cache, "fork", follow_fork)
+    monkeypatch.setattr(engine.cache, "reorder", follow_reorder)
+    found = engine.beam_search([prompt], 8, beams)[0]
+    assert shared_steps == [False] + [share] * 7
+    # the contents: within the bfloat16 bound of their own sequence's logits, beyond it of the others'
+    # (nearly any: rows of two sequences that end alike may be as near)
+    plain = {ids: logits_of(list(ids)) for ids in rows}
+    apart = []
+    for ids, row in rows.items():
+        for other, want in plain.items():
+            off = (row - want).abs().max().item() / want.abs().max().item()
+            if other == ids:
+                assert off <= BF16_MAX_REL, (len(ids), off)
+            elif len(other) == len(ids):
+                apart.append(off > BF16_MAX_REL)
+    assert sum(apart) >= 0.9 * len(apart) > 0
+    # the choice: scores go on from step to step as float32 (half a step of 2^-24), each total off by up to
+    # 2e-6 (the fast sums) before it is rounded
+    want = plain_search(lambda ids: rows[tuple(ids)], prompt, beams, 8, -1, 1.0)
+    assert [h.token_ids for h in found] == [tokens for _, tokens in want]
+    for h, (score, tokens) in zip(found, want):
+        assert abs(h.score - score) <= 8 * (2e-6 + 2.0 ** -24 * abs(score * len(tokens)))
+
+
 def _architecture(name, root):
     """(folder, last logits of a sequence, a prompt) of a small model of each architecture."""
     import importlib
