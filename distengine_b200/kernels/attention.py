@@ -126,7 +126,8 @@ class AttentionLauncher:
         self._sm_count: "int | None" = None                 # asked of the device at first use
         self.key = (f"attention/{'mma' if self.tensor_cores else 'simt'}/{self.group}/"
                     f"{kv_heads}/{head_dim}/{self.window}"
-                    + ("/exact" if self.tensor_cores and exact_weights else ""))
+                    + ("/exact" if self.tensor_cores and exact_weights else "")
+                    + ("/share" if self.shared is not None else ""))
 
     def _blocks_per_sm(self) -> int:
         """Blocks an SM holds at once: one of the tcgen05 kernel (it takes nearly all shared

@@ -176,3 +176,27 @@ def test_the_plan_says_how_tiles_of_8_rows_go():
                                         seq_pos0=np.array(pos0, dtype=np.int32)))
         launcher.prepare(prep)
         assert prep.notes.get(launcher.key + "/by_tiles") is note
+
+
+@pytest.mark.parametrize("first", [0, 1])
+def test_launchers_that_do_not_share_plan_for_themselves(first):
+    """Beside a launcher of the same heads whose step goes through the shared prefixes."""
+    from types import SimpleNamespace
+
+    import torch
+
+    from distengine_b200.kernels.attention import AttentionLauncher
+    from distengine_b200.parts.context import StepPrep
+    launchers = [AttentionLauncher(torch.float32, 32, 4, 64, 0.125, None, share=True),
+                 AttentionLauncher(torch.float32, 32, 4, 64, -0.125, None, share=True),
+                 AttentionLauncher(torch.float32, 32, 4, 64, 0.125, None)]
+    launchers[0].shared._sms = SMS
+    host = SimpleNamespace(seq_qlen=np.ones(16, dtype=np.int32), seq_slot=np.arange(16, dtype=np.int32),
+                           seq_pos0=np.full(16, 9000, dtype=np.int32), shared=([16], [8992]))
+    for launcher in launchers[first:] + launchers[:first]:
+        prep = StepPrep(host) if launcher is launchers[first] else prep
+        launcher.prepare(prep)
+    for launcher in launchers:
+        assert (prep.notes.get(launcher.key + "/shared") is not None) == (launcher is launchers[0])
+    for launcher in launchers[1:]:
+        assert sum(len(prep.extra[f"{launcher.key}/{s.name}/items"]) for s in launcher.shapes) >= 16
