@@ -308,9 +308,9 @@ class SharedPrefixAttention:
         bounded wait that ran out sets it to 3.  ``buffer(name, shape, dtype)``: where the partial results
         lie during the call (None: fresh memory)."""
         d, heads, kv_heads, tokens = self.head_dim, self.heads, self.kv_heads, plan.tokens
-        _need(plan.group == self.group and plan.kv_heads == kv_heads,
-              f"shared prefix: the plan is one for {plan.kv_heads} kv heads of {plan.group} query heads "
-              f"each, the layer has {kv_heads} of {self.group}")
+        if plan.group != self.group or plan.kv_heads != kv_heads:
+            raise ValueError(f"shared prefix: the plan is one for {plan.kv_heads} kv heads of {plan.group} "
+                             f"query heads each, the layer has {kv_heads} of {self.group}")
         _need(q.dim() == out.dim() == 2, "shared prefix: q and out have a row a token of the plan")
         _need(k_pages.dim() == 4, "shared prefix: pages must be [pages, kv_heads, page, head_dim]")
         q_shape, (q_stride, q_one) = q.shape, q.stride()
