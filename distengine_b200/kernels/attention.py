@@ -116,9 +116,9 @@ class AttentionLauncher:
         # keys and values that several requests share are read once (kernels.shared_prefix);
         # DISTENGINE_B200_SHARED_PREFIX=0 has every request read them for itself
         self.shared = None
-        if (share and scale > 0 and not window and not exact_weights
+        from .shared_prefix import SharedPrefixAttention, takes_scale
+        if (share and takes_scale(scale) and not window and not exact_weights
                 and os.environ.get("DISTENGINE_B200_SHARED_PREFIX", "1") != "0"):
-            from .shared_prefix import SharedPrefixAttention
             self.shared = SharedPrefixAttention(dtype, heads, kv_heads, head_dim, scale, device)
         self._shared_plan: "tuple | None" = None            # (what it was made for, the plan)
         self._decode_blocks_per_sm: "int | None" = None     # asked of the kernel at first use

@@ -25,6 +25,12 @@ from .ops import _check, _need, _on_device, _status_word, _stream, _tag
 MAX_SPLITS = 256         # ranges that a prefix or a request's own keys are cut into
 
 
+def takes_scale(scale: float) -> bool:
+    """Whether the kernels take this scale: above 0, and within the range of float32's normal numbers also
+    times log2(e)."""
+    return 2.0 ** -126 <= scale <= 2.0 ** 127
+
+
 @dataclass
 class SharedPlan:
     """The work lists of a step's requests: ``items`` by kernel, int32 [n, 8] (``shared_prefix::Item``;
@@ -225,13 +231,13 @@ class SharedPrefixAttention:
 
     def __init__(self, dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int, scale: float,
                  device: "torch.device | str | None" = None) -> None:
-        """``scale`` above 0; float32 or bfloat16, even head sizes up to 256."""
+        """``scale`` above 0 (``takes_scale``); float32 or bfloat16, even head sizes up to 256."""
         check_head_dim(head_dim)
         _tag(dtype)
         if heads <= 0 or kv_heads <= 0 or heads % kv_heads != 0:
             raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
-        if not 0.0 < scale < float("inf"):
-            raise ValueError(f"shared prefix: the scale must be positive, got {scale}")
+        if not takes_scale(scale):
+            raise ValueError(f"shared prefix: the scale must be a positive float32 number, got {scale}")
         self.dtype, self.heads, self.kv_heads, self.head_dim = dtype, heads, kv_heads, head_dim
         self.scale, self.group = float(scale), heads // kv_heads
         self.tensor_cores = uses_tensor_cores(dtype, head_dim)

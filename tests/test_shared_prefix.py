@@ -188,3 +188,14 @@ def test_a_plan_keeps_its_heads():
     tile = TILES["places"][0]
     plan = plan_shared([1, 1], [2], [16], 5, 3, lambda r, k: tile, lambda r, k: tile).to("cpu")
     assert (plan.group, plan.kv_heads, plan.turns) == (5, 3, True)
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-40, 1e39, 1e300])
+def test_scales_that_are_no_float32_numbers_are_refused(scale):
+    """The kernels take it as one: 0 or an infinity would make every result NaN.  A launcher that may share
+    does not then."""
+    from distengine_b200.kernels.attention import AttentionLauncher
+    with pytest.raises(ValueError, match="shared prefix: the scale"):
+        SharedPrefixAttention(torch.float32, 4, 2, 64, scale)
+    assert AttentionLauncher(torch.float32, 4, 2, 64, scale, None, share=True).shared is None
+    SharedPrefixAttention(torch.float32, 4, 2, 64, 1e-30)
