@@ -15,15 +15,16 @@
 //     o += p v (p in tensor memory, v MN-major straight from the pages);
 //   * warps 18 and 19 fetch: a ring of buffers of 128 keys or 128 values, one TMA box a page and 64 features.
 // A tile goes through in halves of 64 keys, each with columns of tensor memory of its own, so a half's scores
-// are formed while the other's exponentials are (512 rows behind 65,003 keys 151 us; tiles of 128 keys at a
-// time, whose scores had to wait for the weights over them, 171).  A row's exponentials refer to a maximum
-// that is raised, and o rescaled, only when a score has grown by more than 2^8 beyond it.
+// are formed while the other's exponentials are (512 rows behind 65,003 keys, on one GPU at 1,965 MHz, 151 us;
+// tiles of 128 keys at a time, whose scores had to wait for the weights over them, 171).  A row's exponentials
+// refer to a maximum that is raised, and o rescaled, only when a score has grown by more than 2^8 beyond it.
 //
 // What bounds it: with r rows a block a byte of keys and values takes r multiply-adds, so up to 128 rows
 // it is the cache's way from memory (at head size 128: 108 rows behind 15,566 keys of 32 kv heads, 255 MB, 53 us
 // of the call's 76), beyond it the tensor cores and, as much, the exponentials: 128 x 128 scores take the
-// tensor cores 1,024 cycles at head size 128 and 512 at 64, their exponentials 1,024 (16 a cycle); 512 rows
-// behind 65,003 keys run at 880 TFLOP/s.
+// tensor cores 1,024 cycles at head size 128 and 512 at 64, their exponentials 1,024 (16 a cycle).  512 rows
+// behind 65,003 keys: a call now and then 155 to 160 us (870 TFLOP/s at 1,965 MHz), call after call 184 (740;
+// the power limit of 1,000 W then leaves the SMs 1,580 MHz).
 //
 // Every wait is bounded (status 3; the block then stores no result, runs to its end and frees its tensor
 // memory).  One block an SM.

@@ -789,9 +789,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, best: torch.Tensor, 
     the ``take`` largest, best first, with their beams and tokens.
 
     logits float32 [groups * beams, vocabulary] (row stride free), scores float32 [groups, beams];
-    best float32, beam and token int32, all [groups, take]; up to 32 beams, 64 taken.  Totals are formed
-    and compared in 64 bits; of equal ones the lower beam comes first, within a beam the larger logit,
-    then the lower token.  A total of minus infinity or NaN (a masked token, a dead beam, a row that
+    best float32, beam and token int32, all [groups, take]; up to 32 beams, 64 taken.  Which are taken, and
+    in which order, is as in 64 bits; of equal totals the lower beam comes first, within a beam the larger
+    logit, then the lower token.  ``best`` may be off by 1.1e-6, from a sum of float32 exponentials, before
+    it is rounded to float32 (the sums are formed anew only where they decide an order).  A total of minus infinity or NaN (a masked token, a dead beam, a row that
     holds NaN or plus infinity) is no candidate; where too few are left, best is minus infinity and
     beam and token are -1.  ``scratch``: uint8, ``beam_scratch`` bytes, used during the call."""
     _need(logits.dim() == scores.dim() == best.dim() == 2,
